@@ -387,6 +387,74 @@ NE_API ne_status ne_rmsnorm_bwd_add(ne_ctx* ctx, const float* d_dy, const float*
 NE_API ne_status ne_sdpa_fwd_device(ne_ctx* ctx, const void* d_q, const void* d_k,
                                     const void* d_v, int B, int S, void* d_out, float* d_lse);
 
+/* ---- losses of the head ---------------------------------------------------
+ * Softmax cross entropy and distillation from a teacher's top logits, straight
+ * from hidden states x [rows, dim] and the head's weight w [vocab, dim] on
+ * caller-owned device buffers (bf16; any weight, e.g. the tied embedding).
+ * The logits z = scale * x . w^T are made a piece of the vocabulary at a time
+ * and never kept.  Counterpart of the classifier and cross_entropy_loss
+ * (train.m:495-523, cpu_ops.h:348-382); distillation and the left-out rows
+ * have none there.
+ *
+ * All calls only enqueue work on the context's stream, use the workspaces of
+ * ne_head_alloc and may be captured into a graph.  dim, ldx, ldw, lddx and
+ * lddw are multiples of 8, x, w, dx and dw 16-byte aligned; rows, vocab and
+ * topk are arbitrary (rows may be 0).  Outputs are the same bits every time.
+ * A target or id >= vocab counts as absent and is reported by the next call
+ * that synchronises (NE_ERR_BOUNDS). */
+typedef struct ne_head_desc {
+  const void* x; long long ldx;   /* bf16 [rows, dim]: hidden states after the final norm */
+  const void* w; long long ldw;   /* bf16 [vocab, dim] */
+  int rows, dim, vocab;
+  float scale;                    /* of the logits; positive (1 for the models here) */
+} ne_head_desc;
+
+/* A teacher's largest logits: topk (1 .. 256) entries per row, in any order;
+ * an entry with id < 0 or a logit of -inf is absent (its logit or id is not
+ * looked at further), and an id that stands twice in a row counts as the sum
+ * of its probabilities. */
+typedef struct ne_teacher_desc {
+  const int32_t* ids;    /* device [rows, topk] */
+  const float* logits;   /* device [rows, topk] */
+  int topk;
+  float temperature;     /* T > 0: both sides' logits are divided by it */
+} ne_teacher_desc;
+
+/* Gradients to compute (NULL: not computed).  dx [rows, dim] is written, bf16
+ * or (dx_f32) fp32, zeros in left-out rows.  dw [vocab, dim]: bf16 is written,
+ * fp32 (dw_f32) is added to, as the training gradients accumulate. */
+typedef struct ne_head_grads {
+  void* dx; long long lddx; int dx_f32;
+  void* dw; long long lddw; int dw_f32;
+} ne_head_grads;
+
+/* Workspaces for calls of up to these sizes (max_topk 0: cross entropy only).
+ * A later call with larger sizes waits for the stream and allocates anew, which
+ * invalidates graphs captured before; one that fits does nothing. */
+NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_vocab, int max_topk);
+
+/* d_loss[i] = lse_i - z[i, target_i], d_lse[i] = log sum_v exp z[i, v] (fp32
+ * [rows]).  A row with target < 0 is left out: loss and lse 0, whatever x
+ * holds there.  rows = 1 is one generated token's log-probability (-loss). */
+NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
+                                float* d_loss, float* d_lse);
+/* Gradients of sum_i grad_i loss_i, from the d_lse of ne_head_ce_fwd; d_grad
+ * [rows] NULL: ones.  dz = grad (softmax - onehot) is rounded to bf16 as the
+ * operand of the tensor-core products that give dx and dw. */
+NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
+                                const float* d_lse, const float* d_grad, const ne_head_grads* g);
+
+/* With p = softmax(teacher logits / T) over a row's entries and q =
+ * softmax(z / T) over the vocabulary: d_loss[i] = T^2 sum_k p_k (log p_k - log
+ * q_{id_k}), d_lse[i] = log sum_v exp(z[i, v] / T).  A row without entries is
+ * left out. */
+NE_API ne_status ne_head_distill_fwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
+                                     float* d_loss, float* d_lse);
+/* As ne_head_ce_bwd, with dz = grad T (q - p). */
+NE_API ne_status ne_head_distill_bwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
+                                     const float* d_lse, const float* d_grad,
+                                     const ne_head_grads* g);
+
 /* ---- data-parallel gradients (NCCL over NVLink; no reference counterpart:
  * the reference trains on one device) ---------------------------------------
  * Rank 0 makes an id with ne_comm_unique_id and shares it out of band; every

@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "gemm_tc.cuh"
+#include "gemm_tmap.h"
 #include "ne_internal.h"
 #include "ne_launch.cuh"
 
@@ -33,8 +34,8 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 2-D K-major operand [rows, K] (leading dim ld elements), 128B-swizzled box
-// of 64 x box_rows.
+}  // namespace
+
 bool make_tmap(CUtensorMap* tm, const void* ptr, int rows, int K, long long ld, int box_rows,
                int fp16) {
   EncodeTiledFn enc = encode_fn();
@@ -50,8 +51,6 @@ bool make_tmap(CUtensorMap* tm, const void* ptr, int rows, int K, long long ld, 
   return r == CUDA_SUCCESS;
 }
 
-// 2-D MN-major operand: global [K rows, MN] (MN contiguous, leading dim ld),
-// boxes of 64 (MN) x 64 (K rows), 128B-swizzled.
 bool make_tmap_mn(CUtensorMap* tm, const void* ptr, int mn, int K, long long ld) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
@@ -65,9 +64,6 @@ bool make_tmap_mn(CUtensorMap* tm, const void* ptr, int mn, int K, long long ld)
   return r == CUDA_SUCCESS;
 }
 
-// Output of a staged epilogue: [rows, cols] row-major with leading dim ld
-// elements, boxes of box_cols x 32 rows whose 32-, 64- or 128-byte rows use
-// the matching swizzle (the kernel writes the box in that layout).
 bool make_tmap_out(CUtensorMap* tm, void* ptr, int rows, int cols, long long ld,
                    CUtensorMapDataType dt, int elem_bytes, int box_cols) {
   EncodeTiledFn enc = encode_fn();
@@ -85,6 +81,8 @@ bool make_tmap_out(CUtensorMap* tm, void* ptr, int rows, int cols, long long ld,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
+
+namespace {
 
 // A staged epilogue needs a 16-byte aligned output base and row pitch.
 bool stage_ok(const void* out, long long ld, int elem_bytes) {
@@ -385,6 +383,8 @@ cudaError_t gemm_run(const GemmCall& c, int* status, cudaStream_t st) {
   sh.kb_per_split = kb / splits;
   sh.status = status;
   sh.prefetch_a = c.prefetch_a;
+  sh.d_rows = nullptr;
+  sh.dyn_k = 0;
   // Raster groups when A outgrows a share of L2: M-fastest order re-reads all
   // of A for every wave of n-tiles once A no longer stays resident, so the
   // units run in groups of m-tiles whose A panels total ~48 MB (the wave's B

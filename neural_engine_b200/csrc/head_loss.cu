@@ -1,0 +1,921 @@
+// head_loss.cu -- losses of the language-model head straight from the hidden
+// states, over a vocabulary that is walked in pieces: no logits are kept.
+//
+//   z_iv = scale * x_i . w_v                       x [rows, dim], w [vocab, dim], bf16
+//   cross entropy:   lse_i = log sum_v exp z_iv,   loss_i = lse_i - z_{i,t_i}
+//                    dz_iv = g_i (exp(z_iv - lse_i) - [v = t_i])
+//   distillation:    u = z / T,  p_i = softmax of the teacher's K logits / T
+//                    loss_i = T^2 sum_k p_ik (log p_ik - u_{i,c_ik} + lse_i)
+//                    dz_iv = g_i T (exp(u_iv - lse_i) - sum_{k: c_ik = v} p_ik)
+//   dx_i = scale sum_v dz_iv w_v,   dw_v = scale sum_i dz_iv x_i
+//
+// Cross entropy is the one-entry case of the same product: a dense softmax
+// minus a sparse target.  So both run on
+//   pack      rows that count, moved together (masked rows cost no product and
+//             what stands in them, NaN included, reaches nothing)
+//   teacher   p and the ids of each row, sorted and without repeats (distillation)
+//   forward   x . w^T on the tensor cores; the epilogue keeps per row a running
+//             maximum and sum of exp2 and picks out the target's logits
+//   join      the tiles' (maximum, sum) pairs of a row -> lse, loss
+//   backward  per piece of the vocabulary: the logits again, turned into bf16 dz
+//             by the epilogue, then dx += dz . w and dw = dz^T . x
+// Everything is ordered by the stream and by tiles: no atomics, the same bits
+// every time.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "../../include/ne.h"
+#include "gemm_tc.cuh"
+#include "gemm_tmap.h"
+#include "ne_ctx.h"
+#include "ne_internal.h"
+#include "ne_launch.cuh"
+
+namespace ne {
+
+// Workspaces of the head losses (ne_head_alloc), sized for the largest call.
+struct HeadState {
+  long long max_rows = 0, max_vocab = 0;
+  int max_dim = 0, max_topk = 0;
+  size_t dz_elems = 0;
+  void* pool = nullptr;
+  int* count = nullptr;           // rows that count
+  int* row_of = nullptr;          // packed row -> row, -1 up to the next 64
+  int* pos_of = nullptr;          // row -> packed row, -1 where left out
+  int* keep = nullptr;            // distillation: the row has an entry
+  int* ids = nullptr;             // [topk][rows] sorted, INT_MAX behind the last
+  float* prob = nullptr;          // [topk][rows]
+  float* neg_entropy = nullptr;   // [rows] sum p log p
+  float* zt = nullptr;            // [topk][rows] target logits, log2 units
+  float2* stats = nullptr;        // (max, sum exp2) of each row and half tile
+  __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim] packed x
+  __nv_bfloat16* dz = nullptr;    // one piece of dz
+  float* dx = nullptr;            // [rows up to 64][dim] sum over the pieces
+};
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr int kTopkMax = 256;
+// dz of one piece: small enough that the piece, w's piece and x stay in L2
+// (126 MB) between the product that makes dz and the two that read it
+constexpr size_t kPieceBytes = 64u << 20;
+
+inline long long up(long long n, long long to) { return (n + to - 1) / to * to; }
+
+// ------------------------------------------------------------------ epilogues
+// The sparse targets of a row: sorted ids, [entry][row].
+struct HeadTargets {
+  const int* ids;
+  const float* prob;     // backward: the probability of each id (NULL: 1)
+  const int* row_of;     // NULL: rows are not packed
+  long long ld;          // between entries
+  int n;                 // entries a row
+};
+
+struct TargetCursor {
+  int row, at, next;     // row (-1: none), entry, its id
+};
+
+__device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& c, int m, int M,
+                                            int col0) {
+  c.row = m < M ? (t.row_of ? t.row_of[m] : m) : -1;
+  c.at = 0;
+  c.next = INT_MAX;
+  if (c.row < 0) return;
+  const int* ids = t.ids + c.row;
+  int lo = 0, hi = t.n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ids[mid * t.ld] < col0) lo = mid + 1;
+    else hi = mid;
+  }
+  c.at = lo;
+  if (lo < t.n) c.next = ids[lo * t.ld];
+}
+__device__ __forceinline__ void cursor_step(const HeadTargets& t, TargetCursor& c) {
+  ++c.at;
+  c.next = c.at < t.n ? t.ids[c.at * t.ld + c.row] : INT_MAX;
+}
+
+// Forward: a thread owns one row of the tile and half of its column chunks.
+// It keeps the running maximum m and sum s of exp2(c2 * acc - m), c2 = scale /
+// (T ln 2), in fp32 registers, and writes one pair a tile: 8 bytes for 128
+// logits.
+struct EpiHeadLse {
+  struct Params {
+    HeadTargets t;
+    float2* stats;
+    long long part_stride, row_stride;
+    float* zt;
+    float c2;
+  };
+  struct State {
+    float mx, sum;
+    TargetCursor c;
+  };
+  __device__ static void begin(const Params& p, State& st, int m, int col0, int M) {
+    st.mx = kLowest;
+    st.sum = 0.f;
+    cursor_seek(p.t, st.c, m, M, col0);
+  }
+  template <int CH>
+  __device__ static void chunk(const Params& p, State& st, int, int n0, const float (&v)[CH], int,
+                               int N) {
+    if (st.c.row < 0 || n0 >= N) return;
+    float top = kLowest;
+    if (n0 + CH <= N) {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) top = fmaxf(top, v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+        if (n0 + j < N) top = fmaxf(top, v[j]);
+    }
+    const float mx = fmaxf(st.mx, top * p.c2);
+    float s0 = st.sum * ex2_fast(st.mx - mx), s1 = 0.f;
+    if (n0 + CH <= N) {
+#pragma unroll
+      for (int j = 0; j < CH; j += 2) {
+        s0 += ex2_fast(fmaf(v[j], p.c2, -mx));
+        s1 += ex2_fast(fmaf(v[j + 1], p.c2, -mx));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+        if (n0 + j < N) s0 += ex2_fast(fmaf(v[j], p.c2, -mx));
+    }
+    st.mx = mx;
+    st.sum = s0 + s1;
+    while (st.c.next < n0 + CH) {
+      if (st.c.next >= n0) {
+        const int j = st.c.next - n0;
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          if (i == j) z = v[i];
+        p.zt[st.c.at * p.t.ld + st.c.row] = z * p.c2;
+      }
+      cursor_step(p.t, st.c);
+    }
+  }
+  __device__ static void end(const Params& p, State& st, int m, int nt, int half, int) {
+    if (st.c.row >= 0)
+      p.stats[(2 * nt + half) * p.part_stride + m * p.row_stride] = make_float2(st.mx, st.sum);
+  }
+};
+// the same over packed rows, whose number stands in device memory
+struct EpiHeadLseDyn : EpiHeadLse {
+  static constexpr int kDyn = 1;
+};
+
+// Backward: dz = a (exp2(c2 acc - lse2) - p) of a chunk, a = g T scale, rounded
+// once to bf16: it is the operand of two tensor-core products, whose sums over
+// rows or ids are fp32.  Rows behind the last packed one are written as zeros
+// up to the next 64, the block the dw product reduces over.
+struct EpiHeadDz {
+  static constexpr int kDyn = 1;
+  static constexpr int kStage = 1;
+  static constexpr int kCols = 32;
+  using Out = uint16_t;
+  struct Params {
+    HeadTargets t;
+    const float* lse;
+    const float* grad;    // NULL: 1
+    float c2, factor;     // factor = T * scale
+    int col0;             // the piece's first id
+  };
+  struct State {
+    float a, lse2;
+    TargetCursor c;
+  };
+  __device__ static int out_col(const Params&, int n0) { return n0; }
+  __device__ static void begin(const Params& p, State& st, int m, int n0, int M) {
+    cursor_seek(p.t, st.c, m, M, p.col0 + n0);
+    st.a = st.lse2 = 0.f;
+    if (st.c.row >= 0) {
+      st.lse2 = p.lse[st.c.row] * kLog2e;
+      st.a = (p.grad ? p.grad[st.c.row] : 1.0f) * p.factor;
+    }
+  }
+  template <int CH>
+  __device__ static void stage(const Params& p, State& st, int, int n0, const float (&v)[CH],
+                               Out (&o)[kCols], int, int) {
+    float d[CH];
+    const bool live = st.c.row >= 0;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+      d[j] = live ? st.a * ex2_fast(fmaf(v[j], p.c2, -st.lse2)) : 0.f;
+    const int col = p.col0 + n0;
+    while (st.c.next < col + CH) {
+      if (st.c.next >= col) {
+        const int j = st.c.next - col;
+        const float q = p.t.prob ? p.t.prob[st.c.at * p.t.ld + st.c.row] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          if (i == j) d[i] -= st.a * q;
+      }
+      cursor_step(p.t, st.c);
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) o[j] = __bfloat16_as_ushort(__float2bfloat16_rn(d[j]));
+  }
+  __device__ static void end(const Params&, State&, int, int, int, int) {}
+};
+
+// The gradient products over packed rows.
+struct EpiHeadF32 : EpiF32S { static constexpr int kDyn = 1; };
+struct EpiHeadAdd : EpiResidS { static constexpr int kDyn = 1; };
+struct EpiHeadBF16 : EpiBF16S { static constexpr int kDyn = 1; };
+
+// ------------------------------------------------------------------ rows
+__device__ __forceinline__ bool row_counts(const int32_t* target, const int* keep, int i, int vocab) {
+  if (keep) return keep[i] != 0;
+  const int t = target[i];
+  return t >= 0 && t < vocab;
+}
+
+// Moves the rows that count together, in order.  A block takes 32 rows; how
+// many count before them it counts itself (the targets stay in L2: 4 bytes a
+// row, once per block), so there is no scan to wait for.
+constexpr int PACK_ROWS = 32;
+__global__ void __launch_bounds__(256) head_pack_kernel(
+    const __nv_bfloat16* __restrict__ x, long long ldx, int rows, int dim,
+    const int32_t* __restrict__ target, const int* __restrict__ keep, int vocab, int* row_of,
+    int* pos_of, int* count, __nv_bfloat16* xp, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int before, base_s;
+  __shared__ unsigned mask_s;
+  const int first = blockIdx.x * PACK_ROWS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) before = 0;
+  __syncthreads();
+  int n = 0;
+  for (int i = threadIdx.x; i < first; i += 256) n += row_counts(target, keep, i, vocab);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0 && n) atomicAdd(&before, n);
+  __syncthreads();
+  if (warp == 0) {
+    const int i = first + lane;
+    const bool on = i < rows && row_counts(target, keep, i, vocab);
+    if (!keep && i < rows && target[i] >= vocab) atomicExch(status, DEV_ERR_BOUNDS);
+    const unsigned mask = __ballot_sync(0xffffffffu, on);
+    const int pos = before + __popc(mask & ((1u << lane) - 1));
+    if (i < rows) pos_of[i] = on ? pos : -1;
+    if (on) row_of[pos] = i;
+    if (lane == 0) {
+      mask_s = mask;
+      base_s = before;
+    }
+  }
+  __syncthreads();
+  const unsigned mask = mask_s;
+  const int vecs = dim / 8;
+  for (int r = warp; r < PACK_ROWS; r += 8) {
+    if (!((mask >> r) & 1u)) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(first + r) * ldx);
+    uint4* dst = reinterpret_cast<uint4*>(
+        xp + (long long)(base_s + __popc(mask & ((1u << r) - 1))) * dim);
+    for (int k = lane; k < vecs; k += 32) dst[k] = src[k];
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    const int total = base_s + __popc(mask);
+    const int stop = total > 64 ? (total + 63) / 64 * 64 : 64;
+    if (threadIdx.x == 0) *count = total;
+    for (int i = total + threadIdx.x; i < stop; i += 256) row_of[i] = -1;
+    uint4* z = reinterpret_cast<uint4*>(xp + (long long)total * dim);
+    for (long long k = threadIdx.x; k < (long long)(stop - total) * vecs; k += 256)
+      z[k] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// One warp per row: the softmax over the row's entries, then its ids sorted
+// with repeats added together (in the order of the entries), K^2 comparisons
+// out of shared memory.
+constexpr int TEACHER_WARPS = 4;
+__global__ void __launch_bounds__(32 * TEACHER_WARPS) head_teacher_kernel(
+    const int32_t* __restrict__ ids_in, const float* __restrict__ logit, int rows, int K, int vocab,
+    float inv_t, int* ids, float* prob, float* neg_entropy, int* keep, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int sid[TEACHER_WARPS][kTopkMax];
+  __shared__ float sp[TEACHER_WARPS][kTopkMax];
+  __shared__ int sfirst[TEACHER_WARPS][kTopkMax];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x * TEACHER_WARPS + w;
+  if (r >= rows) return;
+  const int32_t* id = ids_in + (long long)r * K;
+  const float* y = logit + (long long)r * K;
+  float top = -INFINITY;
+  int any = 0;
+  for (int k = lane; k < K; k += 32) {
+    int c = id[k];
+    if (c >= vocab) atomicExch(status, DEV_ERR_BOUNDS);
+    const float v = y[k] * inv_t;
+    if (c < 0 || c >= vocab || v == -INFINITY) c = INT_MAX;
+    sid[w][k] = c;
+    sp[w][k] = v;
+    if (c != INT_MAX) {
+      any = 1;
+      top = fmaxf(top, v);
+    }
+  }
+  any = __any_sync(0xffffffffu, any);
+  top = warp_max(top);
+  __syncwarp();
+  float sum = 0.f;
+  for (int k = lane; k < K; k += 32)
+    if (sid[w][k] != INT_MAX) sum += expf(sp[w][k] - top);
+  sum = warp_sum(sum);
+  const float lsum = logf(sum);
+  float ent = 0.f;
+  for (int k = lane; k < K; k += 32) {
+    float p = 0.f;
+    if (sid[w][k] != INT_MAX) {
+      const float l = sp[w][k] - top;
+      p = expf(l) / sum;
+      if (p != 0.f) ent += p * (l - lsum);
+    }
+    sp[w][k] = p;
+  }
+  ent = warp_sum(ent);
+  __syncwarp();
+  for (int k = lane; k < K; k += 32) {
+    const int c = sid[w][k];
+    int first = c != INT_MAX;
+    for (int j = 0; j < k; ++j)
+      if (sid[w][j] == c) first = 0;
+    sfirst[w][k] = first;
+  }
+  __syncwarp();
+  int total = 0;
+  for (int k = lane; k < K; k += 32) total += sfirst[w][k];
+  total = __reduce_add_sync(0xffffffffu, total);
+  for (int k = lane; k < K; k += 32) {
+    if (sfirst[w][k]) {
+      const int c = sid[w][k];
+      int rank = 0;
+      float p = 0.f;
+      for (int j = 0; j < K; ++j) {
+        const int cj = sid[w][j];
+        rank += sfirst[w][j] && cj < c;
+        if (cj == c) p += sp[w][j];
+      }
+      ids[(long long)rank * rows + r] = c;
+      prob[(long long)rank * rows + r] = p;
+    }
+    if (k >= total) {
+      ids[(long long)k * rows + r] = INT_MAX;
+      prob[(long long)k * rows + r] = 0.f;
+    }
+  }
+  if (lane == 0) {
+    keep[r] = any;
+    neg_entropy[r] = ent;
+  }
+}
+
+// Joins the (maximum, sum) pairs of a row in a fixed order.  RPB rows a block
+// of 256 threads: 32 where there are many rows (the pairs of 32 rows lie side
+// by side), 1 where there are few (the pairs of one row do).
+struct HeadJoin {
+  const float2* stats;
+  long long part_stride, row_stride;
+  int parts, rows, vocab, n;      // n: entries a row
+  const int* pos_of;              // NULL: rows are not packed
+  const int32_t* target;          // cross entropy
+  const int* keep;                // distillation
+  const int* ids;
+  const float* prob;
+  const float* neg_entropy;
+  const float* zt;
+  float t2;                       // T^2
+  float* loss;
+  float* lse;
+  int* status;
+};
+template <int RPB>
+__global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
+  constexpr int SL = 256 / RPB;
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float smx[SL][RPB], ssum[SL][RPB];
+  const int rl = threadIdx.x % RPB, sl = threadIdx.x / RPB;
+  const int i = blockIdx.x * RPB + rl;
+  const bool in = i < p.rows;
+  bool on = in && row_counts(p.target, p.keep, i, p.vocab);
+  if (in && !p.keep && !p.pos_of && sl == 0 && p.target[i] >= p.vocab)
+    atomicExch(p.status, DEV_ERR_BOUNDS);
+  const int m = in && p.pos_of ? p.pos_of[i] : i;
+  float mx = kLowest, sum = 0.f;
+  if (on) {
+    const float2* s = p.stats + m * p.row_stride;
+    // four loads in flight; pairs of a slice are joined in the order of the tiles
+    int k = sl;
+    for (; k + 3 * SL < p.parts; k += 4 * SL) {
+      float2 q[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) q[u] = s[(k + u * SL) * p.part_stride];
+      const float top = fmaxf(fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), mx);
+      sum *= exp2f(mx - top);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum += q[u].y * exp2f(q[u].x - top);
+      mx = top;
+    }
+    for (; k < p.parts; k += SL) {
+      const float2 q = s[k * p.part_stride];
+      const float top = fmaxf(mx, q.x);
+      sum = sum * exp2f(mx - top) + q.y * exp2f(q.x - top);
+      mx = top;
+    }
+  }
+  smx[sl][rl] = mx;
+  ssum[sl][rl] = sum;
+  __syncthreads();
+  for (int h = SL / 2; h >= 1; h >>= 1) {
+    if (sl < h) {
+      const float a = smx[sl][rl], b = smx[sl + h][rl];
+      const float top = fmaxf(a, b);
+      ssum[sl][rl] = ssum[sl][rl] * exp2f(a - top) + ssum[sl + h][rl] * exp2f(b - top);
+      smx[sl][rl] = top;
+    }
+    __syncthreads();
+  }
+  const float lse2 = smx[0][rl] + log2f(ssum[0][rl]);
+  __syncthreads();
+  float part = 0.f;
+  if (on && p.keep) {
+    for (int k = sl; k < p.n; k += SL) {
+      const float q = p.prob[(long long)k * p.rows + i];
+      if (q != 0.f) part += q * (lse2 - p.zt[(long long)k * p.rows + i]);
+    }
+  }
+  ssum[sl][rl] = part;
+  __syncthreads();
+  if (sl == 0 && in) {
+    float loss = 0.f;
+    if (on && p.keep) {
+      float d = 0.f;
+      for (int u = 0; u < SL; ++u) d += ssum[u][rl];
+      loss = p.t2 * (p.neg_entropy[i] + kLn2 * d);
+    } else if (on) {
+      loss = kLn2 * (lse2 - p.zt[i]);
+    }
+    p.loss[i] = loss;
+    p.lse[i] = on ? kLn2 * lse2 : 0.f;
+  }
+}
+
+// dx of the rows as the caller laid them out; zeros where a row was left out.
+template <class T>
+__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int rows,
+                                                      int dim, const int* __restrict__ pos_of,
+                                                      T* dx, long long ld) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= rows) return;
+  const int pos = pos_of[i];
+  const float4* src = reinterpret_cast<const float4*>(acc + (long long)(pos < 0 ? 0 : pos) * dim);
+  T* dst = dx + (long long)i * ld;
+  for (int k = threadIdx.x & 31; k < dim / 4; k += 32) {
+    const float4 v = pos < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : src[k];
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(dst)[k] = v;
+    } else {
+      uint2 o;
+      *reinterpret_cast<__nv_bfloat162*>(&o.x) = __floats2bfloat162_rn(v.x, v.y);
+      *reinterpret_cast<__nv_bfloat162*>(&o.y) = __floats2bfloat162_rn(v.z, v.w);
+      reinterpret_cast<uint2*>(dst)[k] = o;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ products
+template <int BN, class Epi, int AMN, int BMN, int CG>
+cudaError_t launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
+                           const GemmShape& sh, const typename Epi::Params& p, int num_sms,
+                           cudaStream_t st) {
+  using C = GemmCfg<BN, CG>;
+  constexpr int smem = EpiStage<Epi>::value ? C::SMEM_BYTES_STAGED : C::SMEM_BYTES;
+  auto kern = gemm_tc_kernel<BN, Epi, 1, AMN, BMN, CG>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const long long units = (long long)sh.m_tiles * sh.n_tiles;
+  CUtensorMap td{};
+  if constexpr (CG == 2) {
+    const int grid = (int)(2 * std::min<long long>(units, num_sms / 2));
+    return launch_k_cluster(kern, dim3(grid), dim3(GEMM_THREADS), (size_t)smem, st, 2u, ta, tb, tc,
+                            td, sh, p);
+  } else {
+    const int grid = (int)std::min<long long>(units, num_sms);
+    return launch_k(kern, dim3(grid), dim3(GEMM_THREADS), (size_t)smem, st, ta, tb, tc, td, sh, p);
+  }
+}
+
+GemmShape product_shape(int M, int N, int K, int tile_m, int bn, const int* d_rows, int dyn_k,
+                        int* status) {
+  GemmShape sh{};
+  sh.M = M;
+  sh.N = N;
+  sh.K = K;
+  sh.m_tiles = (M + tile_m - 1) / tile_m;
+  sh.n_tiles = (N + bn - 1) / bn;
+  sh.splits = 1;
+  sh.kb_per_split = (K + GEMM_BK - 1) / GEMM_BK;
+  sh.status = status;
+  sh.d_rows = d_rows;
+  sh.dyn_k = dyn_k;
+  // as gemm_run: m-tiles whose A panels stay in L2 while a wave of tiles reuses them
+  const long long panel = (long long)tile_m * K * 2, budget = 48ll << 20;
+  if (sh.n_tiles > 1 && panel * sh.m_tiles > budget)
+    sh.group_m = (int)std::max<long long>(1, budget / panel);
+  return sh;
+}
+
+// What a call works on, after its arguments were checked.
+struct HeadCall {
+  const ne_head_desc* d;
+  const int32_t* target = nullptr;      // cross entropy
+  const ne_teacher_desc* teacher = nullptr;
+  float t = 1.0f;
+  int n = 1;
+};
+
+ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
+  if (!d->x || !d->w) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x or w is NULL");
+  if (d->rows < 0 || d->dim <= 0 || d->vocab <= 0)
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": rows, dim or vocab out of range");
+  if (d->dim % 8) return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": dim must be a multiple of 8");
+  if (d->ldx < d->dim || d->ldw < d->dim || d->ldx % 8 || d->ldw % 8)
+    return fail(ctx, NE_ERR_INVALID,
+                std::string(what) + ": ldx and ldw must be multiples of 8, at least dim");
+  if ((reinterpret_cast<uintptr_t>(d->x) | reinterpret_cast<uintptr_t>(d->w)) & 15u)
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x and w must be 16-byte aligned");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale))
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": scale must be positive and finite");
+  const HeadState* h = ctx->head;
+  if (!h || d->rows > h->max_rows || d->dim > h->max_dim || d->vocab > h->max_vocab)
+    return fail(ctx, NE_ERR_STATE, std::string(what) + ": ne_head_alloc has no room for this call");
+  return NE_OK;
+}
+
+ne_status teacher_check(ne_ctx* ctx, const ne_teacher_desc* t, const char* what) {
+  if (!t->ids || !t->logits || t->topk <= 0)
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": teacher ids, logits or topk missing");
+  if (t->topk > kTopkMax)
+    return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": topk is at most 256");
+  if (!(t->temperature > 0.f) || !std::isfinite(t->temperature))
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature must be positive and finite");
+  if (t->topk > ctx->head->max_topk)
+    return fail(ctx, NE_ERR_STATE, std::string(what) + ": ne_head_alloc has no room for this topk");
+  return NE_OK;
+}
+
+ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
+  if (!c.teacher) return NE_OK;
+  HeadState* h = ctx->head;
+  const int rows = c.d->rows;
+  NE_LAUNCH(launch_k(head_teacher_kernel, dim3((rows + TEACHER_WARPS - 1) / TEACHER_WARPS),
+                     dim3(32 * TEACHER_WARPS), 0, ctx->st, c.teacher->ids, c.teacher->logits, rows,
+                     c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->neg_entropy, h->keep,
+                     ctx->d_status));
+  return NE_OK;
+}
+
+ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c) {
+  HeadState* h = ctx->head;
+  const int rows = c.d->rows;
+  NE_LAUNCH(launch_k(head_pack_kernel, dim3((rows + PACK_ROWS - 1) / PACK_ROWS), dim3(256), 0,
+                     ctx->st, (const __nv_bfloat16*)c.d->x, c.d->ldx, rows, c.d->dim, c.target,
+                     (const int*)(c.teacher ? h->keep : nullptr), c.d->vocab, h->row_of, h->pos_of,
+                     h->count, h->xp, ctx->d_status));
+  return NE_OK;
+}
+
+HeadTargets targets_of(const HeadState* h, const HeadCall& c, bool packed) {
+  HeadTargets t{};
+  t.ids = c.teacher ? h->ids : c.target;
+  t.prob = c.teacher ? h->prob : nullptr;
+  t.row_of = packed ? h->row_of : nullptr;
+  t.ld = c.d->rows;
+  t.n = c.n;
+  return t;
+}
+
+ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) {
+  HeadState* h = ctx->head;
+  const ne_head_desc& d = *c.d;
+  const int rows = d.rows, V = d.vocab, D = d.dim, sms = ctx->num_sms;
+  ne_status s;
+  if ((s = enqueue_teacher(ctx, c)) != NE_OK) return s;
+  // up to one tile of rows, nothing is saved by packing
+  const bool packed = rows > GEMM_BM;
+  const bool pair = rows >= 512;
+  const int bn = packed ? 256 : 64;
+  if (packed && (s = enqueue_pack(ctx, c)) != NE_OK) return s;
+  EpiHeadLse::Params p{};
+  p.t = targets_of(h, c, packed);
+  p.stats = h->stats;
+  const int parts = 2 * ((V + bn - 1) / bn);
+  p.part_stride = packed ? rows : 1;
+  p.row_stride = packed ? 1 : parts;
+  p.zt = h->zt;
+  p.c2 = d.scale / c.t * kLog2e;
+  const int tile_m = pair ? 2 * GEMM_BM : GEMM_BM;
+  const GemmShape sh = product_shape(rows, V, D, tile_m, bn, h->count, 0, ctx->d_status);
+  CUtensorMap ta, tb, tc{};
+  if (!make_tmap(&ta, packed ? h->xp : d.x, rows, D, packed ? D : d.ldx, GEMM_BM, 0) ||
+      !make_tmap(&tb, d.w, V, D, d.ldw, pair ? bn / 2 : bn, 0))
+    return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
+  if (pair)
+    NE_LAUNCH((launch_product<256, EpiHeadLseDyn, 0, 0, 2>(ta, tb, tc, sh, p, sms, ctx->st)));
+  else if (packed)
+    NE_LAUNCH((launch_product<256, EpiHeadLseDyn, 0, 0, 1>(ta, tb, tc, sh, p, sms, ctx->st)));
+  else
+    NE_LAUNCH((launch_product<64, EpiHeadLse, 0, 0, 1>(ta, tb, tc, sh, p, sms, ctx->st)));
+  HeadJoin j{};
+  j.stats = h->stats;
+  j.part_stride = p.part_stride;
+  j.row_stride = p.row_stride;
+  j.parts = parts;
+  j.rows = rows;
+  j.vocab = V;
+  j.n = c.n;
+  j.pos_of = packed ? h->pos_of : nullptr;
+  j.target = c.target;
+  j.keep = c.teacher ? h->keep : nullptr;
+  j.ids = h->ids;
+  j.prob = h->prob;
+  j.neg_entropy = h->neg_entropy;
+  j.zt = h->zt;
+  j.t2 = c.t * c.t;
+  j.loss = loss;
+  j.lse = lse;
+  j.status = ctx->d_status;
+  if (packed)
+    NE_LAUNCH(launch_k(head_join_kernel<32>, dim3((rows + 31) / 32), dim3(256), 0, ctx->st, j));
+  else
+    NE_LAUNCH(launch_k(head_join_kernel<1>, dim3(rows), dim3(256), 0, ctx->st, j));
+  return NE_OK;
+}
+
+ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const float* grad,
+                        const ne_head_grads* g) {
+  HeadState* h = ctx->head;
+  const ne_head_desc& d = *c.d;
+  const int rows = d.rows, V = d.vocab, D = d.dim, sms = ctx->num_sms;
+  const int rows64 = (int)up(rows, 64);
+  ne_status s;
+  if ((s = enqueue_teacher(ctx, c)) != NE_OK || (s = enqueue_pack(ctx, c)) != NE_OK) return s;
+  const bool pair = rows >= 512;
+  const int tile_m = pair ? 2 * GEMM_BM : GEMM_BM;
+  // equal pieces of whole 256-id tiles, as few as the room for dz allows
+  const long long room = std::max<long long>(256, (long long)(kPieceBytes / 2) / rows64 / 256 * 256);
+  const int pieces = (int)((V + room - 1) / room);
+  const int piece = (int)up((V + pieces - 1) / pieces, 256);
+  for (int v0 = 0; v0 < V; v0 += piece) {
+    const int nv = std::min(piece, V - v0);
+    const int ldz = (int)up(nv, 64);
+    const __nv_bfloat16* w = (const __nv_bfloat16*)d.w + (long long)v0 * d.ldw;
+    CUtensorMap ta, tb, tc;
+    // dz = f(x . w^T)
+    if (!make_tmap(&ta, h->xp, rows64, D, D, GEMM_BM, 0) ||
+        !make_tmap(&tb, w, nv, D, d.ldw, pair ? 128 : 256, 0) ||
+        !make_tmap_out(&tc, h->dz, rows64, nv, ldz, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 32))
+      return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
+    EpiHeadDz::Params pz{};
+    pz.t = targets_of(h, c, true);
+    pz.lse = lse;
+    pz.grad = grad;
+    pz.c2 = d.scale / c.t * kLog2e;
+    pz.factor = c.t * d.scale;
+    pz.col0 = v0;
+    GemmShape sh = product_shape(rows, nv, D, tile_m, 256, h->count, 0, ctx->d_status);
+    if (pair) NE_LAUNCH((launch_product<256, EpiHeadDz, 0, 0, 2>(ta, tb, tc, sh, pz, sms, ctx->st)));
+    else NE_LAUNCH((launch_product<256, EpiHeadDz, 0, 0, 1>(ta, tb, tc, sh, pz, sms, ctx->st)));
+    if (g->dx) {   // dx (+)= dz . w
+      if (!make_tmap(&ta, h->dz, rows64, nv, ldz, GEMM_BM, 0) ||
+          !make_tmap_mn(&tb, w, D, nv, d.ldw) ||
+          !make_tmap_out(&tc, h->dx, rows64, D, D, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 32))
+        return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
+      sh = product_shape(rows, D, nv, tile_m, 256, h->count, 0, ctx->d_status);
+      const EpiF32S::Params ps{0};
+      const EpiResidS::Params pa{1.0f};
+      if (v0 == 0 && pair)
+        NE_LAUNCH((launch_product<256, EpiHeadF32, 0, 1, 2>(ta, tb, tc, sh, ps, sms, ctx->st)));
+      else if (v0 == 0)
+        NE_LAUNCH((launch_product<256, EpiHeadF32, 0, 1, 1>(ta, tb, tc, sh, ps, sms, ctx->st)));
+      else if (pair)
+        NE_LAUNCH((launch_product<256, EpiHeadAdd, 0, 1, 2>(ta, tb, tc, sh, pa, sms, ctx->st)));
+      else
+        NE_LAUNCH((launch_product<256, EpiHeadAdd, 0, 1, 1>(ta, tb, tc, sh, pa, sms, ctx->st)));
+    }
+    if (g->dw) {   // dw = dz^T . x
+      const int esz = g->dw_f32 ? 4 : 2;
+      void* out = (uint8_t*)g->dw + (long long)v0 * g->lddw * esz;
+      const bool wide = nv >= 512;
+      if (!make_tmap_mn(&ta, h->dz, nv, rows64, ldz) || !make_tmap_mn(&tb, h->xp, D, rows64, D) ||
+          !make_tmap_out(&tc, out, nv, D, g->lddw,
+                         g->dw_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                         esz, 32))
+        return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
+      sh = product_shape(nv, D, rows, wide ? 256 : 128, 256, h->count, 1, ctx->d_status);
+      const EpiBF16S::Params pb{1.0f, 0};
+      const EpiResidS::Params pa{1.0f};
+      if (g->dw_f32 && wide)
+        NE_LAUNCH((launch_product<256, EpiHeadAdd, 1, 1, 2>(ta, tb, tc, sh, pa, sms, ctx->st)));
+      else if (g->dw_f32)
+        NE_LAUNCH((launch_product<256, EpiHeadAdd, 1, 1, 1>(ta, tb, tc, sh, pa, sms, ctx->st)));
+      else if (wide)
+        NE_LAUNCH((launch_product<256, EpiHeadBF16, 1, 1, 2>(ta, tb, tc, sh, pb, sms, ctx->st)));
+      else
+        NE_LAUNCH((launch_product<256, EpiHeadBF16, 1, 1, 1>(ta, tb, tc, sh, pb, sms, ctx->st)));
+    }
+  }
+  if (g->dx) {
+    const dim3 grid((rows + 7) / 8);
+    if (g->dx_f32)
+      NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
+                         rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx));
+    else
+      NE_LAUNCH(launch_k(head_dx_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->st,
+                         (const float*)h->dx, rows, D, (const int*)h->pos_of, (__nv_bfloat16*)g->dx,
+                         g->lddx));
+  }
+  return NE_OK;
+}
+
+ne_status grads_check(ne_ctx* ctx, const ne_head_desc* d, const ne_head_grads* g, const char* what) {
+  if (!g->dx && !g->dw) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": no gradient asked for");
+  if ((g->dx && (g->lddx < d->dim || g->lddx % 8)) || (g->dw && (g->lddw < d->dim || g->lddw % 8)))
+    return fail(ctx, NE_ERR_INVALID,
+                std::string(what) + ": lddx and lddw must be multiples of 8, at least dim");
+  if ((reinterpret_cast<uintptr_t>(g->dx) | reinterpret_cast<uintptr_t>(g->dw)) & 15u)
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": dx and dw must be 16-byte aligned");
+  return NE_OK;
+}
+
+// No rows: dw of no rows is zero where it is written, and stays where it is added to.
+ne_status no_rows(ne_ctx* ctx, const ne_head_desc* d, const ne_head_grads* g) {
+  if (g->dw && !g->dw_f32)
+    NE_CUDA(cudaMemset2DAsync(g->dw, (size_t)g->lddw * 2, 0, (size_t)d->dim * 2, (size_t)d->vocab,
+                              ctx->st));
+  return NE_OK;
+}
+
+}  // namespace
+
+void free_head(ne_ctx* ctx) {
+  if (!ctx->head) return;
+  if (ctx->head->pool) cudaFree(ctx->head->pool);
+  delete ctx->head;
+  ctx->head = nullptr;
+}
+
+}  // namespace ne
+
+using namespace ne;
+
+extern "C" {
+
+NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_vocab, int max_topk) {
+  if (!ctx) return NE_ERR_INVALID;
+  if (max_rows <= 0 || max_dim <= 0 || max_vocab <= 0 || max_topk < 0)
+    return fail(ctx, NE_ERR_INVALID, "ne_head_alloc: sizes out of range");
+  if (max_dim % 8) return fail(ctx, NE_ERR_UNSUPPORTED, "ne_head_alloc: dim must be a multiple of 8");
+  if (max_topk > kTopkMax) return fail(ctx, NE_ERR_UNSUPPORTED, "ne_head_alloc: topk is at most 256");
+  if (max_rows > (1 << 22))
+    return fail(ctx, NE_ERR_UNSUPPORTED, "ne_head_alloc: at most 4194304 rows a call");
+  HeadState n;
+  n.max_rows = max_rows;
+  n.max_dim = max_dim;
+  n.max_vocab = max_vocab;
+  n.max_topk = max_topk;
+  if (const HeadState* o = ctx->head) {
+    if (max_rows <= o->max_rows && max_dim <= o->max_dim && max_vocab <= o->max_vocab &&
+        max_topk <= o->max_topk)
+      return NE_OK;
+    n.max_rows = std::max(n.max_rows, o->max_rows);
+    n.max_dim = std::max(n.max_dim, o->max_dim);
+    n.max_vocab = std::max(n.max_vocab, o->max_vocab);
+    n.max_topk = std::max(n.max_topk, o->max_topk);
+  }
+  NE_CUDA(cudaSetDevice(ctx->device));
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  NE_CUDA(cudaStreamIsCapturing(ctx->st, &cs));
+  if (cs != cudaStreamCaptureStatusNone)
+    return fail(ctx, NE_ERR_STATE, "ne_head_alloc inside a capture");
+  NE_CUDA(cudaStreamSynchronize(ctx->st));
+  free_head(ctx);
+  const size_t R = n.max_rows, R256 = up(R, 256), D = n.max_dim, V = n.max_vocab;
+  const size_t K = std::max(n.max_topk, 1);
+  // a piece is at least 256 ids wide, whatever the rows
+  n.dz_elems = std::max<size_t>(kPieceBytes / 2, up(R, 64) * 256);
+  n.dz_elems = std::min<size_t>(n.dz_elems, up(R, 64) * up(V, 256));
+  // pairs: two a 256-id tile and row; up to one tile of rows, two a 64-id tile
+  const size_t pairs = std::max(2 * ((V + 255) / 256) * R,
+                                2 * ((V + 63) / 64) * std::min<size_t>(R, GEMM_BM));
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off += up(bytes, 1024);
+    return at;
+  };
+  const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4),
+               o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
+               o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8),
+               o_xp = take(R256 * D * 2), o_dz = take(n.dz_elems * 2), o_dx = take(up(R, 64) * D * 4);
+  uint8_t* b = nullptr;
+  ne_status s = dalloc(ctx, &b, off);
+  if (s != NE_OK) return s;
+  n.pool = b;
+  n.count = (int*)(b + o_count);
+  n.row_of = (int*)(b + o_row);
+  n.pos_of = (int*)(b + o_pos);
+  n.keep = (int*)(b + o_keep);
+  n.ids = (int*)(b + o_ids);
+  n.prob = (float*)(b + o_prob);
+  n.neg_entropy = (float*)(b + o_ent);
+  n.zt = (float*)(b + o_zt);
+  n.stats = (float2*)(b + o_stats);
+  n.xp = (__nv_bfloat16*)(b + o_xp);
+  n.dz = (__nv_bfloat16*)(b + o_dz);
+  n.dx = (float*)(b + o_dx);
+  ctx->head = new HeadState(n);
+  return NE_OK;
+}
+
+NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
+                                float* d_loss, float* d_lse) {
+  if (!ctx || !d) return NE_ERR_INVALID;
+  if (!d_target || !d_loss || !d_lse)
+    return fail(ctx, NE_ERR_INVALID, "ne_head_ce_fwd: target, loss or lse is NULL");
+  ne_status s = head_check(ctx, d, "ne_head_ce_fwd");
+  if (s != NE_OK || d->rows == 0) return s;
+  NE_CUDA(cudaSetDevice(ctx->device));
+  HeadCall c;
+  c.d = d;
+  c.target = d_target;
+  return head_forward(ctx, c, d_loss, d_lse);
+}
+
+NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
+                                const float* d_lse, const float* d_grad, const ne_head_grads* g) {
+  if (!ctx || !d || !g) return NE_ERR_INVALID;
+  if (!d_target || !d_lse)
+    return fail(ctx, NE_ERR_INVALID, "ne_head_ce_bwd: target or lse is NULL");
+  ne_status s = head_check(ctx, d, "ne_head_ce_bwd");
+  if (s != NE_OK || (s = grads_check(ctx, d, g, "ne_head_ce_bwd")) != NE_OK) return s;
+  NE_CUDA(cudaSetDevice(ctx->device));
+  if (d->rows == 0) return no_rows(ctx, d, g);
+  HeadCall c;
+  c.d = d;
+  c.target = d_target;
+  return head_backward(ctx, c, d_lse, d_grad, g);
+}
+
+NE_API ne_status ne_head_distill_fwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
+                                     float* d_loss, float* d_lse) {
+  if (!ctx || !d || !t) return NE_ERR_INVALID;
+  if (!d_loss || !d_lse)
+    return fail(ctx, NE_ERR_INVALID, "ne_head_distill_fwd: loss or lse is NULL");
+  ne_status s = head_check(ctx, d, "ne_head_distill_fwd");
+  if (s != NE_OK || (s = teacher_check(ctx, t, "ne_head_distill_fwd")) != NE_OK || d->rows == 0)
+    return s;
+  NE_CUDA(cudaSetDevice(ctx->device));
+  HeadCall c;
+  c.d = d;
+  c.teacher = t;
+  c.t = t->temperature;
+  c.n = t->topk;
+  return head_forward(ctx, c, d_loss, d_lse);
+}
+
+NE_API ne_status ne_head_distill_bwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
+                                     const float* d_lse, const float* d_grad,
+                                     const ne_head_grads* g) {
+  if (!ctx || !d || !t || !g) return NE_ERR_INVALID;
+  if (!d_lse) return fail(ctx, NE_ERR_INVALID, "ne_head_distill_bwd: lse is NULL");
+  ne_status s = head_check(ctx, d, "ne_head_distill_bwd");
+  if (s != NE_OK || (s = teacher_check(ctx, t, "ne_head_distill_bwd")) != NE_OK ||
+      (s = grads_check(ctx, d, g, "ne_head_distill_bwd")) != NE_OK)
+    return s;
+  NE_CUDA(cudaSetDevice(ctx->device));
+  if (d->rows == 0) return no_rows(ctx, d, g);
+  HeadCall c;
+  c.d = d;
+  c.teacher = t;
+  c.t = t->temperature;
+  c.n = t->topk;
+  return head_backward(ctx, c, d_lse, d_grad, g);
+}
+
+}  // extern "C"

@@ -20,6 +20,8 @@ struct TrainState;                      // ne_train.cu
 void free_train(ne_ctx* ctx);           // ne_train.cu
 struct Comm;                            // comm.cu
 void comm_free(ne_ctx* ctx);            // comm.cu
+struct HeadState;                       // head_loss.cu
+void free_head(ne_ctx* ctx);            // head_loss.cu
 }  // namespace ne
 
 namespace ne {
@@ -53,6 +55,7 @@ struct ne_ctx {
   int launches = 0;  // kernels enqueued by the current enqueue_* call
   ne::TrainState* train = nullptr;  // training buffers (ne_train_alloc)
   ne::Comm* comm = nullptr;         // NCCL gradient exchange (ne_comm_init)
+  ne::HeadState* head = nullptr;    // head-loss workspaces (ne_head_alloc)
   int comm_timeout_ms = 0;          // ne_comm_set_timeout (0: NE_COMM_TIMEOUT_MS or 120 s)
 
   // weights

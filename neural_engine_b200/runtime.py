@@ -37,7 +37,9 @@ EXPORTED = ("ne_init", "ne_free", "ne_last_error", "ne_status_str", "ne_sync", "
             "ne_sdpa_fwd_device", "ne_train_set_vocab_map", "ne_stream_read",
             "ne_comm_set_sharding", "ne_train_gather_state", "ne_train_fwd_bwd_timed",
             "ne_train_value_ranges", "ne_comm_set_timeout", "ne_shard_range",
-            "ne_gemm_dw_owned", "ne_ckpt_probe", "ne_fault_calls")
+            "ne_gemm_dw_owned", "ne_ckpt_probe", "ne_fault_calls",
+            "ne_head_alloc", "ne_head_ce_fwd", "ne_head_ce_bwd", "ne_head_distill_fwd",
+            "ne_head_distill_bwd")
 
 def shard_range(n: int, world: int, rank: int, lib=None):
     """(offset, length) of the part of an n-element tensor that `rank` owns
@@ -103,6 +105,21 @@ class GemmDescC(C.Structure):
                 ("out", C.c_void_p), ("ld", C.c_longlong), ("alpha", C.c_float),
                 ("aux0", C.c_void_p), ("aux1", C.c_void_p), ("aux_ld", C.c_longlong),
                 ("bn", C.c_int), ("half_out", C.c_int)]
+
+
+class HeadDescC(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("ldx", C.c_longlong), ("w", C.c_void_p), ("ldw", C.c_longlong),
+                ("rows", C.c_int), ("dim", C.c_int), ("vocab", C.c_int), ("scale", C.c_float)]
+
+
+class TeacherDescC(C.Structure):
+    _fields_ = [("ids", C.c_void_p), ("logits", C.c_void_p), ("topk", C.c_int),
+                ("temperature", C.c_float)]
+
+
+class HeadGradsC(C.Structure):
+    _fields_ = [("dx", C.c_void_p), ("lddx", C.c_longlong), ("dx_f32", C.c_int),
+                ("dw", C.c_void_p), ("lddw", C.c_longlong), ("dw_f32", C.c_int)]
 
 
 class AdamCfgC(C.Structure):
@@ -228,6 +245,12 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
     lib.ne_lr_schedule.argtypes = [I, F, I, I, F]
     lib.ne_lr_schedule.restype = F
     lib.ne_train_get_layer.argtypes = [P, I, I] + [P] * 11
+    H, T, G = C.POINTER(HeadDescC), C.POINTER(TeacherDescC), C.POINTER(HeadGradsC)
+    lib.ne_head_alloc.argtypes = [P, I, I, I, I]
+    lib.ne_head_ce_fwd.argtypes = [P, H, P, P, P]
+    lib.ne_head_ce_bwd.argtypes = [P, H, P, P, P, G]
+    lib.ne_head_distill_fwd.argtypes = [P, H, T, P, P]
+    lib.ne_head_distill_bwd.argtypes = [P, H, T, P, P, G]
     lib.ne_stream_read.argtypes = [P, C.c_longlong, P, P]
     _lib = lib
     return lib
@@ -330,6 +353,57 @@ class Engine:
         self._check(self.lib.ne_sdpa_fwd_device(self._ctx, C.c_void_p(d_q), C.c_void_p(d_k),
                                                 C.c_void_p(d_v), int(B), int(S), C.c_void_p(d_out),
                                                 C.c_void_p(d_lse) if d_lse else None))
+
+    # -- losses of the head (pointers are device addresses): cross entropy and
+    #    distillation from x [rows, dim] and w [vocab, dim], logits never kept
+    def head_alloc(self, max_rows: int, max_dim: int, max_vocab: int, max_topk: int = 0):
+        """Room for head-loss calls of up to these sizes (max_topk 0: cross entropy only)."""
+        self._check(self.lib.ne_head_alloc(self._ctx, int(max_rows), int(max_dim), int(max_vocab),
+                                           int(max_topk)))
+
+    @staticmethod
+    def _head(x, w, rows, dim, vocab, scale, ldx, ldw):
+        return HeadDescC(x, ldx or dim, w, ldw or dim, rows, dim, vocab, scale)
+
+    @staticmethod
+    def _head_grads(dim, dx, dw, lddx, lddw, dx_f32, dw_f32):
+        return HeadGradsC(dx, lddx or dim, int(bool(dx_f32)), dw, lddw or dim, int(bool(dw_f32)))
+
+    def head_ce_fwd(self, x: int, w: int, rows: int, dim: int, vocab: int, target: int, loss: int,
+                    lse: int, scale: float = 1.0, ldx: int = 0, ldw: int = 0):
+        """Row losses and log-sum-exps of softmax cross entropy; target < 0 leaves a row out."""
+        d = self._head(x, w, rows, dim, vocab, scale, ldx, ldw)
+        self._check(self.lib.ne_head_ce_fwd(self._ctx, C.byref(d), target, loss, lse))
+
+    def head_ce_bwd(self, x: int, w: int, rows: int, dim: int, vocab: int, target: int, lse: int,
+                    grad: int | None = None, dx: int | None = None, dw: int | None = None,
+                    scale: float = 1.0, ldx: int = 0, ldw: int = 0, lddx: int = 0, lddw: int = 0,
+                    dx_f32: bool = False, dw_f32: bool = False):
+        """Gradients of sum(grad * loss): dx written, dw written (bf16) or added to (fp32)."""
+        d = self._head(x, w, rows, dim, vocab, scale, ldx, ldw)
+        g = self._head_grads(dim, dx, dw, lddx, lddw, dx_f32, dw_f32)
+        self._check(self.lib.ne_head_ce_bwd(self._ctx, C.byref(d), target, lse, grad, C.byref(g)))
+
+    def head_distill_fwd(self, x: int, w: int, rows: int, dim: int, vocab: int, ids: int,
+                         teacher: int, topk: int, loss: int, lse: int, temperature: float = 1.0,
+                         scale: float = 1.0, ldx: int = 0, ldw: int = 0):
+        """Row losses T^2 KL(teacher's topk || softmax(z / T)) and log-sum-exps of z / T; an
+        entry with id < 0 is absent, a row without entries is left out."""
+        d = self._head(x, w, rows, dim, vocab, scale, ldx, ldw)
+        t = TeacherDescC(ids, teacher, topk, temperature)
+        self._check(self.lib.ne_head_distill_fwd(self._ctx, C.byref(d), C.byref(t), loss, lse))
+
+    def head_distill_bwd(self, x: int, w: int, rows: int, dim: int, vocab: int, ids: int,
+                         teacher: int, topk: int, lse: int, grad: int | None = None,
+                         dx: int | None = None, dw: int | None = None, temperature: float = 1.0,
+                         scale: float = 1.0, ldx: int = 0, ldw: int = 0, lddx: int = 0,
+                         lddw: int = 0, dx_f32: bool = False, dw_f32: bool = False):
+        """Gradients of sum(grad * loss) of head_distill_fwd, as head_ce_bwd gives them."""
+        d = self._head(x, w, rows, dim, vocab, scale, ldx, ldw)
+        t = TeacherDescC(ids, teacher, topk, temperature)
+        g = self._head_grads(dim, dx, dw, lddx, lddw, dx_f32, dw_f32)
+        self._check(self.lib.ne_head_distill_bwd(self._ctx, C.byref(d), C.byref(t), lse, grad,
+                                                 C.byref(g)))
 
     # -- data-parallel gradient exchange (NCCL)
     @staticmethod
