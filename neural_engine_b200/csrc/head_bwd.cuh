@@ -1,0 +1,526 @@
+// head_bwd.cuh -- one step of the head losses' backward pass: the three
+// products of a piece of the vocabulary in one persistent launch.
+//
+//   dz[p]  = f(x . w[p]^T)              rows x piece, K = dim
+//   dx    += dz[p-1] . w[p-1]           rows x dim,   K = piece (in splits)
+//   dw[p-1] = dz[p-1]^T . x             piece x dim,  K = rows
+//
+// Step p makes dz of piece p and uses that of piece p - 1, so the three have no
+// order among them and share the SMs: on their own they leave 14% of the pairs
+// idle in the last wave (4096 rows, dim 1024: 64 tiles of dx or 128 of dw for 74
+// pairs) and pay a launch each.  Work units are one 128 * CG x 256 tile (dx: of
+// one split of the piece); the leading CTA's producer draws them from a counter
+// in device memory, the longest kind first, and hands them to the other roles
+// of both CTAs through a ring of slots.  Which pair computes a unit changes no
+// value: every unit is computed whole, and what units of different steps add
+// into is ordered by the launches.
+//
+// Shared-memory ring, TMEM accumulators and CTA pairs are those of gemm_tc.cuh,
+// and so are the warp roles but for the producer: issuing a tensor load takes a
+// thread 110 to 150 cycles and the MMA of a k-block 512, so one warp loads A
+// (and draws the units), another B.
+#pragma once
+#include "gemm_tc.cuh"
+
+namespace ne {
+
+constexpr int HB_BN = 256;
+constexpr int HB_SLOTS = 4;
+constexpr int HB_THREADS = GEMM_THREADS + 32;   // warps: A, MMA, 8 x epilogue, B
+
+struct HeadStep {
+  const int* d_rows;        // packed rows
+  int* counter;             // next work unit, zero at launch
+  int* status;
+  int rows64;               // slab height of dx
+  int dim, dim_kb, dim_tiles;   // dim, in k-blocks of 64 and in tiles of 256
+  // piece p (dz): first id, ids (0: none)
+  int make0, make_n;
+  // piece p - 1 (dx, dw): first id, ids (0: none), ids per dx split (a multiple of 64)
+  int use0, use_n, split_n, splits;
+  int want_dx, want_dw, dx_add, dw_f32;
+};
+
+// The sparse targets of a row: sorted ids, [entry][row].
+struct HeadTargets {
+  const int* ids;
+  const float* prob;     // backward: the probability of each id (NULL: 1)
+  const int* row_of;     // NULL: rows are not packed
+  long long ld;          // between entries
+  int n;                 // entries a row
+};
+
+struct TargetCursor {
+  int row, at, next;     // row (-1: none), entry, its id
+};
+
+__device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& c, int m, int M,
+                                            int col0) {
+  c.row = m < M ? (t.row_of ? t.row_of[m] : m) : -1;
+  c.at = 0;
+  c.next = 0x7fffffff;
+  if (c.row < 0) return;
+  const int* ids = t.ids + c.row;
+  int lo = 0, hi = t.n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ids[mid * t.ld] < col0) lo = mid + 1;
+    else hi = mid;
+  }
+  c.at = lo;
+  if (lo < t.n) c.next = ids[lo * t.ld];
+}
+__device__ __forceinline__ void cursor_step(const HeadTargets& t, TargetCursor& c) {
+  ++c.at;
+  c.next = c.at < t.n ? t.ids[c.at * t.ld + c.row] : 0x7fffffff;
+}
+
+// What turns logits into dz = a (exp2(c2 acc - lse2) - p), a = g T scale.
+struct HeadDz {
+  HeadTargets t;
+  const float* lse;
+  const float* grad;    // NULL: 1
+  float c2, factor;     // scale / (T ln 2), T * scale
+};
+
+struct HeadMaps {
+  CUtensorMap x_k, w_k;        // dz: operands (K = dim contiguous)
+  CUtensorMap dz_out;          // dz: piece p
+  CUtensorMap dz_k, w_mn;      // dx: dz of piece p - 1 (K = ids), w as [ids][dim]
+  CUtensorMap dx_out;          // dx: [splits * rows64][dim] fp32
+  CUtensorMap dz_mn, x_mn;     // dw: both as [rows][...]
+  CUtensorMap dw_out;
+};
+
+enum HeadKind : int { HK_DX = 0, HK_DW = 1, HK_DZ = 2 };
+
+struct HeadUnit {
+  int kind, mt, nt, split, kb0, kb;
+};
+
+// unit u of the step, dx first (the longest), dz last
+__device__ __forceinline__ bool head_unit(const HeadStep& s, int rows_blocks, int m_tiles, int tile_m,
+                                          int u, HeadUnit& o) {
+  const int n_dx = s.use_n && s.want_dx ? m_tiles * s.dim_tiles * s.splits : 0;
+  o.split = 0;
+  o.kb0 = 0;
+  if (u < n_dx) {
+    o.kind = HK_DX;
+    o.nt = u % s.dim_tiles;
+    const int r = u / s.dim_tiles;
+    o.mt = r % m_tiles;
+    o.split = r / m_tiles;
+    o.kb0 = o.split * (s.split_n / GEMM_BK);
+    const int left = s.use_n - o.split * s.split_n;
+    o.kb = (min(left, s.split_n) + GEMM_BK - 1) / GEMM_BK;
+    return true;
+  }
+  u -= n_dx;
+  const int v_tiles = (s.use_n + tile_m - 1) / tile_m;
+  const int n_dw = s.want_dw ? v_tiles * s.dim_tiles : 0;
+  if (u < n_dw) {
+    o.kind = HK_DW;
+    o.nt = u % s.dim_tiles;
+    o.mt = u / s.dim_tiles;
+    o.kb = rows_blocks;
+    return true;
+  }
+  u -= n_dw;
+  if (u < m_tiles * ((s.make_n + HB_BN - 1) / HB_BN)) {
+    o.kind = HK_DZ;
+    o.mt = u % m_tiles;
+    o.nt = u / m_tiles;
+    o.kb = s.dim_kb;
+    return true;
+  }
+  return false;
+}
+
+// Arrivals and writes across the pair.  The data that crosses is one int a work
+// unit, written together with its completion (st.async), so nothing has to be
+// fenced at cluster scope: such a release costs an epilogue warp about 1,400
+// cycles, and the matching acquire another 1,000.
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void post_int(uint32_t cluster_addr, uint32_t cluster_bar, int v) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], 4;" ::"r"(
+                   cluster_bar)
+               : "memory");
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(
+          cluster_addr),
+      "r"(v), "r"(cluster_bar)
+      : "memory");
+}
+
+// 32 values to bf16, the low 16 bits of each word first.
+__device__ __forceinline__ void pack_bf16(const float (&v)[32], uint32_t* o) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    o[j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// This lane's row of a box of 32 rows of 128 bytes, in the 128-byte swizzle.
+__device__ __forceinline__ void stage_words(uint32_t box, int lane, const uint32_t (&o)[32]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    st_shared_v4(box + lane * 128 + ((q ^ (lane & 7)) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2],
+                 o[4 * q + 3]);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+        "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+        "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+        "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int CG>
+__global__ void __launch_bounds__(HB_THREADS, 1)
+head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const HeadDz dzp) {
+  using C = GemmCfg<HB_BN, CG>;
+  constexpr bool PAIR = CG == 2;
+  constexpr int TILE_M = GEMM_BM * CG;
+  constexpr int STAGES = C::STAGES;
+  constexpr uint32_t MN_BOX = 64 * GEMM_BK * 2;
+  constexpr int B_ROWS = HB_BN / CG;
+  // readers of a slot: the MMA thread, B's producer and 8 epilogue warps, and the
+  // other CTA's producers and epilogue warps
+  constexpr int SLOT_READERS = CG * (2 + GEMM_EPI_WARPS);
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const gbase = smem_raw + (base - raw);
+  const uint32_t tiles = base;
+  const uint32_t bars = base + STAGES * C::STAGE_BYTES;
+  const uint32_t full_bar = bars;                         // [STAGES]
+  const uint32_t empty_bar = full_bar + 8 * STAGES;       // [STAGES]
+  const uint32_t tfull_bar = empty_bar + 8 * STAGES;      // [2]
+  const uint32_t tempty_bar = tfull_bar + 16;             // [2]
+  const uint32_t drain_bar = tempty_bar + 16;             // [1]
+  const uint32_t sfull_bar = drain_bar + 8;               // [HB_SLOTS]
+  const uint32_t sempty_bar = sfull_bar + 8 * HB_SLOTS;   // [HB_SLOTS], the leader's
+  const uint32_t slots = sempty_bar + 8 * HB_SLOTS;       // [HB_SLOTS] int
+  const uint32_t misc = slots + 4 * HB_SLOTS;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + (misc - base));
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + (misc - base) + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t crank = PAIR ? cluster_ctarank() : 0u;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar + 8 * s, 1);
+      mbar_init(empty_bar + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar + 8 * a, 1);
+      mbar_init(tempty_bar + 8 * a, CG * GEMM_EPI_WARPS);
+    }
+    mbar_init(drain_bar, 1);
+    for (int s = 0; s < HB_SLOTS; ++s) {
+      mbar_init(sfull_bar + 8 * s, 1);
+      mbar_init(sempty_bar + 8 * s, SLOT_READERS);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), C::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  // whole blocks of 64 rows, at least one (its rows are zeros)
+  const int blocks = max((*sp.d_rows + GEMM_BK - 1) / GEMM_BK, 1);
+  const int M = blocks * GEMM_BK;
+  const int m_tiles = (M + TILE_M - 1) / TILE_M;
+
+  // a role other than the leader's producer takes the unit of slot `it`
+  auto take = [&](int it, int& u) -> bool {
+    const int s = it % HB_SLOTS;
+    if (!mbar_wait(sfull_bar + 8 * s, (it / HB_SLOTS) & 1, sp.status, abort_flag)) return false;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(slots + 4 * s) : "memory");
+    return true;
+  };
+  auto taken = [&](int it) {
+    const uint32_t b = sempty_bar + 8 * (it % HB_SLOTS);
+    if constexpr (PAIR) mbar_arrive_peer(mapa_shared(b, 0));
+    else mbar_arrive(b);
+  };
+
+  if (warp == 0 || warp == 2 + GEMM_EPI_WARPS) {
+    // ------------------------------------------------ TMA producers
+    if (lane == 0) {
+      const bool is_a = warp == 0;
+      const bool leads = is_a && (!PAIR || crank == 0);   // draws the units, arms the barriers
+      const uint64_t pol = policy_evict_normal();
+      // pair mode: all loads of both CTAs complete on the even CTA's barriers
+      const uint32_t full_to = PAIR ? mapa_shared(full_bar, 0) : full_bar;
+      auto ld = [&](uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
+        if constexpr (PAIR) tma_load_2d_pair(dst, tm, bar, c0, c1, pol);
+        else tma_load_2d(dst, tm, bar, c0, c1, pol);
+      };
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int drawn = leads ? atomicAdd(sp.counter, 1) : 0;
+      for (int it = 0; ok; ++it) {
+        int u;
+        if (leads) {
+          u = drawn;
+          const int s = it % HB_SLOTS;
+          if (!mbar_wait(sempty_bar + 8 * s, ((it / HB_SLOTS) & 1) ^ 1, sp.status, abort_flag)) break;
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(slots + 4 * s), "r"(u) : "memory");
+          mbar_arrive(sfull_bar + 8 * s);
+          if constexpr (PAIR) post_int(mapa_shared(slots + 4 * s, 1), mapa_shared(sfull_bar + 8 * s, 1), u);
+        } else {
+          if (!take(it, u)) break;
+          taken(it);
+        }
+        HeadUnit w;
+        if (!head_unit(sp, blocks, m_tiles, TILE_M, u, w)) break;
+        if (leads) drawn = atomicAdd(sp.counter, 1);   // its latency passes behind the loads
+        // this role's operand: K-major is one box, MN-major one per 64 columns
+        const bool mn = is_a ? w.kind == HK_DW : w.kind != HK_DZ;
+        const CUtensorMap* tm =
+            is_a ? (w.kind == HK_DZ ? &maps.x_k : w.kind == HK_DX ? &maps.dz_k : &maps.dz_mn)
+                 : (w.kind == HK_DZ ? &maps.w_k : w.kind == HK_DX ? &maps.w_mn : &maps.x_mn);
+        // first row (K-major) or column (MN-major) of the tile, and where K starts
+        const int first = is_a ? w.mt * TILE_M + (int)crank * GEMM_BM
+                               : w.nt * HB_BN + (int)crank * B_ROWS + (w.kind == HK_DZ ? sp.make0 : 0);
+        int k0 = w.kb0 * GEMM_BK + (!is_a && w.kind == HK_DX ? sp.use0 : 0);
+        for (int k = 0; k < w.kb; ++k, k0 += GEMM_BK) {
+          const uint32_t bar = full_to + 8 * stage;
+          const uint32_t dst = tiles + stage * C::STAGE_BYTES + (is_a ? 0 : C::A_BYTES);
+          if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, sp.status, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (leads) mbar_arrive_expect_tx(full_bar + 8 * stage, CG * C::STAGE_BYTES);
+          if (!mn) {
+            ld(dst, tm, bar, k0, first);
+          } else {
+            ld(dst, tm, bar, first, k0);
+            ld(dst + MN_BOX, tm, bar, first + 64, k0);
+            if (!PAIR && !is_a) {   // 256 rows of B in one CTA
+              ld(dst + 2 * MN_BOX, tm, bar, first + 128, k0);
+              ld(dst + 3 * MN_BOX, tm, bar, first + 192, k0);
+            }
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // no load may be in flight when the CTA exits (gemm_tc.cuh)
+      if (leads) {
+        for (int s = 0; s < STAGES; ++s) {
+          const uint32_t par = (s < stage) ? phase : (phase ^ 1u);
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(full_bar + 8 * s, par)) {
+            if (globaltimer_ns() - t0 > 100000000ull) break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0 && (!PAIR || crank == 0)) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int acc = 0;
+      uint32_t acc_phase = 0;
+      for (int it = 0;; ++it) {
+        int u;
+        if (!take(it, u)) break;
+        taken(it);
+        HeadUnit w;
+        if (!head_unit(sp, blocks, m_tiles, TILE_M, u, w)) break;
+        if (!mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, sp.status, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * HB_BN;
+        const int a_mn = w.kind == HK_DW, b_mn = w.kind != HK_DZ;
+        const uint32_t idesc = umma_idesc_f16(TILE_M, HB_BN, 1) | ((uint32_t)a_mn << 15) |
+                               ((uint32_t)b_mn << 16);
+        const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+        bool ok = true;
+        for (int k = 0; k < w.kb; ++k) {
+          if (!mbar_wait(full_bar + 8 * stage, phase, sp.status, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = tiles + stage * C::STAGE_BYTES;
+          const uint64_t ad = a_mn ? smem_desc_mn_sw128(sa, MN_BOX) : smem_desc_k_sw128(sa);
+          const uint64_t bd = b_mn ? smem_desc_mn_sw128(sa + C::A_BYTES, MN_BOX)
+                                   : smem_desc_k_sw128(sa + C::A_BYTES);
+#pragma unroll
+          for (int j = 0; j < GEMM_BK / 16; ++j)
+            if constexpr (PAIR)
+              umma_f16_pair(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
+            else
+              umma_f16(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
+          if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
+          else umma_commit(empty_bar + 8 * stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
+        else umma_commit(tfull_bar + 8 * acc);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+      if constexpr (PAIR) umma_commit_pair(drain_bar, 0x1);
+      else umma_commit(drain_bar);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain_bar, 0)) {
+        if (globaltimer_ns() - t0 > 100000000ull) break;
+      }
+    }
+  } else {
+    // ------------------------------------------------ epilogue (warps 2..9)
+    const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const uint32_t sbuf = base + STAGES * C::STAGE_BYTES + 1024 + (warp - 2) * GEMM_STAGE_SLOT;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int it = 0;; ++it) {
+      int u = 0;
+      const bool got = take(it, u);
+      if (!__all_sync(0xffffffffu, got)) break;
+      __syncwarp();
+      if (lane == 0) taken(it);
+      HeadUnit w;
+      if (!head_unit(sp, blocks, m_tiles, TILE_M, u, w)) break;
+      const int y0 = w.mt * TILE_M + (int)crank * GEMM_BM + quarter * 32;   // the warp's first row
+      const int n_tile = w.nt * HB_BN;
+      // |dz| = 2^(c2 acc - lse2 + log2|a|) - |a| p: the coefficient goes into the
+      // exponent, its sign and the rows that do not count into two masks
+      TargetCursor cur;
+      float mag = 0.f, shift = 0.f;
+      uint32_t keep = 0u, sign = 0u;
+      if (w.kind == HK_DZ) {
+        cursor_seek(dzp.t, cur, y0 + lane, M, sp.make0 + n_tile + 128 * half);
+        if (cur.row >= 0) {
+          const float a = (dzp.grad ? dzp.grad[cur.row] : 1.0f) * dzp.factor;
+          mag = fabsf(a);
+          shift = __log2f(mag) - dzp.lse[cur.row] * 1.4426950408889634f;
+          keep = 0xffffffffu;
+          sign = a < 0.f ? 0x80008000u : 0u;
+        }
+      }
+      const bool ready = mbar_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * HB_BN;
+      const bool b16 = w.kind == HK_DZ || (w.kind == HK_DW && !sp.dw_f32);
+      const bool rows_in = y0 < (w.kind == HK_DW ? sp.use_n : M);
+      const int cols_end = w.kind == HK_DZ ? sp.make_n : sp.dim;
+      const CUtensorMap* out = w.kind == HK_DZ ? &maps.dz_out
+                               : w.kind == HK_DW ? &maps.dw_out : &maps.dx_out;
+      // a warp owns half of the tile's columns and sends 128-byte rows: 64
+      // columns of bf16 or 32 of fp32 at a time
+      const int step = b16 ? 64 : 32;
+      const bool add = w.kind == HK_DX ? sp.dx_add : w.kind == HK_DW && sp.dw_f32;
+      const int y = w.kind == HK_DX ? w.split * sp.rows64 + y0 : y0;
+#pragma unroll 1
+      for (int c = 128 * half; c < 128 * half + 128; c += step) {
+        const int n0 = n_tile + c;
+        uint32_t o[32];
+        if (b16) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            tmem_ld32(t_row + c + 32 * h, v);
+            if (w.kind == HK_DZ) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
+              const int col = sp.make0 + n0 + 32 * h;
+              while (cur.next < col + 32) {
+                if (cur.next >= col) {
+                  const int j = cur.next - col;
+                  const float q = dzp.t.prob ? dzp.t.prob[cur.at * dzp.t.ld + cur.row] : 1.0f;
+#pragma unroll
+                  for (int i = 0; i < 32; ++i)
+                    if (i == j) v[i] -= mag * q;
+                }
+                cursor_step(dzp.t, cur);
+              }
+            }
+            // rounded once to bf16: dz is the operand of two tensor-core
+            // products, dw the caller's type
+            pack_bf16(v, o + 16 * h);
+          }
+          if (w.kind == HK_DZ) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
+          }
+        } else {
+          float v[32];
+          tmem_ld32(t_row + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
+        }
+        if (lane == 0) bulk_wait_read_all();   // the previous box has left the slot
+        __syncwarp();
+        stage_words(sbuf, lane, o);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (rows_in && n0 < cols_end) {
+            if (add) tma_reduce_add_2d(out, sbuf, n0, y);
+            else tma_store_2d(out, sbuf, n0, y);
+          }
+          bulk_commit_group();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_peer(mapa_shared(tempty_bar + 8 * acc, 0));
+        else mbar_arrive(tempty_bar + 8 * acc);
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();
+  tc_fence_after();
+  if (warp == 1) {
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+    else tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+}  // namespace ne

@@ -31,6 +31,7 @@
 #include "../../include/ne.h"
 #include "gemm_tc.cuh"
 #include "gemm_tmap.h"
+#include "head_bwd.cuh"
 #include "ne_ctx.h"
 #include "ne_internal.h"
 #include "ne_launch.cuh"
@@ -41,7 +42,6 @@ namespace ne {
 struct HeadState {
   long long max_rows = 0, max_vocab = 0;
   int max_dim = 0, max_topk = 0;
-  size_t dz_elems = 0;
   void* pool = nullptr;
   int* count = nullptr;           // rows that count
   int* row_of = nullptr;          // packed row -> row, -1 up to the next 64
@@ -53,8 +53,9 @@ struct HeadState {
   float* zt = nullptr;            // [topk][rows] target logits, log2 units
   float2* stats = nullptr;        // (max, sum exp2) of each row and half tile
   __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim] packed x
-  __nv_bfloat16* dz = nullptr;    // one piece of dz
-  float* dx = nullptr;            // [rows up to 64][dim] sum over the pieces
+  __nv_bfloat16* dz[2] = {};      // the pieces of dz that are made and used
+  float* dx = nullptr;            // [splits][rows up to 64][dim] sums over the pieces
+  int* counters = nullptr;        // work units drawn, one per backward step
 };
 
 namespace {
@@ -63,47 +64,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kTopkMax = 256;
-// dz of one piece: small enough that the piece, w's piece and x stay in L2
-// (126 MB) between the product that makes dz and the two that read it
-constexpr size_t kPieceBytes = 64u << 20;
+// dz of one piece (two are alive), and the slabs dx is summed in where its
+// product is split
+constexpr size_t kPieceBytes = 128u << 20;
+constexpr size_t kSlabBytes = 64u << 20;
 
-inline long long up(long long n, long long to) { return (n + to - 1) / to * to; }
+inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-// ------------------------------------------------------------------ epilogues
-// The sparse targets of a row: sorted ids, [entry][row].
-struct HeadTargets {
-  const int* ids;
-  const float* prob;     // backward: the probability of each id (NULL: 1)
-  const int* row_of;     // NULL: rows are not packed
-  long long ld;          // between entries
-  int n;                 // entries a row
-};
-
-struct TargetCursor {
-  int row, at, next;     // row (-1: none), entry, its id
-};
-
-__device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& c, int m, int M,
-                                            int col0) {
-  c.row = m < M ? (t.row_of ? t.row_of[m] : m) : -1;
-  c.at = 0;
-  c.next = INT_MAX;
-  if (c.row < 0) return;
-  const int* ids = t.ids + c.row;
-  int lo = 0, hi = t.n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ids[mid * t.ld] < col0) lo = mid + 1;
-    else hi = mid;
-  }
-  c.at = lo;
-  if (lo < t.n) c.next = ids[lo * t.ld];
-}
-__device__ __forceinline__ void cursor_step(const HeadTargets& t, TargetCursor& c) {
-  ++c.at;
-  c.next = c.at < t.n ? t.ids[c.at * t.ld + c.row] : INT_MAX;
-}
-
+// ------------------------------------------------------------------ forward epilogue
 // Forward: a thread owns one row of the tile and half of its column chunks.
 // It keeps the running maximum m and sum s of exp2(c2 * acc - m), c2 = scale /
 // (T ln 2), in fp32 registers, and writes one pair a tile: 8 bytes for 128
@@ -175,65 +143,6 @@ struct EpiHeadLseDyn : EpiHeadLse {
   static constexpr int kDyn = 1;
 };
 
-// Backward: dz = a (exp2(c2 acc - lse2) - p) of a chunk, a = g T scale, rounded
-// once to bf16: it is the operand of two tensor-core products, whose sums over
-// rows or ids are fp32.  Rows behind the last packed one are written as zeros
-// up to the next 64, the block the dw product reduces over.
-struct EpiHeadDz {
-  static constexpr int kDyn = 1;
-  static constexpr int kStage = 1;
-  static constexpr int kCols = 32;
-  using Out = uint16_t;
-  struct Params {
-    HeadTargets t;
-    const float* lse;
-    const float* grad;    // NULL: 1
-    float c2, factor;     // factor = T * scale
-    int col0;             // the piece's first id
-  };
-  struct State {
-    float a, lse2;
-    TargetCursor c;
-  };
-  __device__ static int out_col(const Params&, int n0) { return n0; }
-  __device__ static void begin(const Params& p, State& st, int m, int n0, int M) {
-    cursor_seek(p.t, st.c, m, M, p.col0 + n0);
-    st.a = st.lse2 = 0.f;
-    if (st.c.row >= 0) {
-      st.lse2 = p.lse[st.c.row] * kLog2e;
-      st.a = (p.grad ? p.grad[st.c.row] : 1.0f) * p.factor;
-    }
-  }
-  template <int CH>
-  __device__ static void stage(const Params& p, State& st, int, int n0, const float (&v)[CH],
-                               Out (&o)[kCols], int, int) {
-    float d[CH];
-    const bool live = st.c.row >= 0;
-#pragma unroll
-    for (int j = 0; j < CH; ++j)
-      d[j] = live ? st.a * ex2_fast(fmaf(v[j], p.c2, -st.lse2)) : 0.f;
-    const int col = p.col0 + n0;
-    while (st.c.next < col + CH) {
-      if (st.c.next >= col) {
-        const int j = st.c.next - col;
-        const float q = p.t.prob ? p.t.prob[st.c.at * p.t.ld + st.c.row] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (i == j) d[i] -= st.a * q;
-      }
-      cursor_step(p.t, st.c);
-    }
-#pragma unroll
-    for (int j = 0; j < CH; ++j) o[j] = __bfloat16_as_ushort(__float2bfloat16_rn(d[j]));
-  }
-  __device__ static void end(const Params&, State&, int, int, int, int) {}
-};
-
-// The gradient products over packed rows.
-struct EpiHeadF32 : EpiF32S { static constexpr int kDyn = 1; };
-struct EpiHeadAdd : EpiResidS { static constexpr int kDyn = 1; };
-struct EpiHeadBF16 : EpiBF16S { static constexpr int kDyn = 1; };
-
 // ------------------------------------------------------------------ rows
 __device__ __forceinline__ bool row_counts(const int32_t* target, const int* keep, int i, int vocab) {
   if (keep) return keep[i] != 0;
@@ -248,9 +157,11 @@ constexpr int PACK_ROWS = 32;
 __global__ void __launch_bounds__(256) head_pack_kernel(
     const __nv_bfloat16* __restrict__ x, long long ldx, int rows, int dim,
     const int32_t* __restrict__ target, const int* __restrict__ keep, int vocab, int* row_of,
-    int* pos_of, int* count, __nv_bfloat16* xp, int* status) {
+    int* pos_of, int* count, __nv_bfloat16* xp, int* counters, int n_counters, int* status) {
   pdl_trigger();
   pdl_wait();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
   __shared__ int before, base_s;
   __shared__ unsigned mask_s;
   const int first = blockIdx.x * PACK_ROWS;
@@ -473,11 +384,13 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
   }
 }
 
-// dx of the rows as the caller laid them out; zeros where a row was left out.
+// dx of the rows as the caller laid them out, the slabs added in their order;
+// zeros where a row was left out.
 template <class T>
-__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int rows,
-                                                      int dim, const int* __restrict__ pos_of,
-                                                      T* dx, long long ld) {
+__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int slabs,
+                                                      long long slab, int rows, int dim,
+                                                      const int* __restrict__ pos_of, T* dx,
+                                                      long long ld) {
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -486,7 +399,14 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
   const float4* src = reinterpret_cast<const float4*>(acc + (long long)(pos < 0 ? 0 : pos) * dim);
   T* dst = dx + (long long)i * ld;
   for (int k = threadIdx.x & 31; k < dim / 4; k += 32) {
-    const float4 v = pos < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : src[k];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (pos >= 0) {
+      v = src[k];
+      for (int u = 1; u < slabs; ++u) {
+        const float4 q = src[k + u * (slab / 4)];
+        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+      }
+    }
     if constexpr (sizeof(T) == 4) {
       reinterpret_cast<float4*>(dst)[k] = v;
     } else {
@@ -590,13 +510,13 @@ ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
   return NE_OK;
 }
 
-ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c) {
+ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, int counters) {
   HeadState* h = ctx->head;
   const int rows = c.d->rows;
   NE_LAUNCH(launch_k(head_pack_kernel, dim3((rows + PACK_ROWS - 1) / PACK_ROWS), dim3(256), 0,
                      ctx->st, (const __nv_bfloat16*)c.d->x, c.d->ldx, rows, c.d->dim, c.target,
                      (const int*)(c.teacher ? h->keep : nullptr), c.d->vocab, h->row_of, h->pos_of,
-                     h->count, h->xp, ctx->d_status));
+                     h->count, h->xp, h->counters, counters, ctx->d_status));
   return NE_OK;
 }
 
@@ -620,7 +540,7 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   const bool packed = rows > GEMM_BM;
   const bool pair = rows >= 512;
   const int bn = packed ? 256 : 64;
-  if (packed && (s = enqueue_pack(ctx, c)) != NE_OK) return s;
+  if (packed && (s = enqueue_pack(ctx, c, 0)) != NE_OK) return s;
   EpiHeadLse::Params p{};
   p.t = targets_of(h, c, packed);
   p.stats = h->stats;
@@ -667,88 +587,126 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   return NE_OK;
 }
 
+// How the backward pass walks the vocabulary.
+struct HeadPlan {
+  int cg, tile_m, clusters;   // CTAs a tile, rows a tile, clusters at once
+  int piece, pieces;          // ids a piece (whole tiles), pieces
+  int split_n, splits;        // ids a split of dx's product
+};
+
+HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
+  HeadPlan p;
+  // one CTA's 128 rows where they are enough, else pairs of CTAs
+  p.cg = rows > GEMM_BM ? 2 : 1;
+  p.tile_m = GEMM_BM * p.cg;
+  p.clusters = num_sms / p.cg;
+  const long long rows64 = up(rows, 64);
+  const long long room = std::max<long long>(HB_BN, (long long)(kPieceBytes / 2) / rows64 / HB_BN * HB_BN);
+  p.pieces = (int)((vocab + room - 1) / room);
+  p.piece = (int)up((vocab + p.pieces - 1) / p.pieces, HB_BN);
+  p.pieces = (vocab + p.piece - 1) / p.piece;
+  // dx's units are the longest: where there are few of them the piece is split
+  // until a unit is at most half of what a pair has to do in a step
+  const double m_tiles = (double)((rows + p.tile_m - 1) / p.tile_m), d_tiles = (dim + HB_BN - 1) / HB_BN;
+  const double piece_kb = p.piece / GEMM_BK;
+  double load = m_tiles * d_tiles * piece_kb + (p.piece / p.tile_m) * d_tiles * (double)(rows64 / GEMM_BK);
+  if (p.pieces > 1) load += m_tiles * (p.piece / HB_BN) * (double)((dim + GEMM_BK - 1) / GEMM_BK);
+  const double most = std::max(8.0, load / p.clusters / 2);
+  const long long slabs = std::max<long long>(1, (long long)kSlabBytes / (rows64 * dim * 4));
+  const long long want = std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
+  p.split_n = (int)up((p.piece + want - 1) / want, GEMM_BK);
+  p.splits = (p.piece + p.split_n - 1) / p.split_n;
+  return p;
+}
+
+template <int CG>
+cudaError_t launch_step(const HeadMaps& maps, const HeadStep& step, const HeadDz& dz, int clusters,
+                        cudaStream_t st) {
+  using C = GemmCfg<HB_BN, CG>;
+  auto kern = head_step_kernel<CG>;
+  const size_t smem = C::SMEM_BYTES_STAGED;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  if constexpr (CG == 2)
+    return launch_k_cluster(kern, dim3(2 * clusters), dim3(HB_THREADS), smem, st, 2u, maps, step, dz);
+  else
+    return launch_k(kern, dim3(clusters), dim3(HB_THREADS), smem, st, maps, step, dz);
+}
+
 ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const float* grad,
                         const ne_head_grads* g) {
   HeadState* h = ctx->head;
   const ne_head_desc& d = *c.d;
-  const int rows = d.rows, V = d.vocab, D = d.dim, sms = ctx->num_sms;
+  const int rows = d.rows, V = d.vocab, D = d.dim;
   const int rows64 = (int)up(rows, 64);
+  const HeadPlan plan = head_plan(rows, D, V, ctx->num_sms);
   ne_status s;
-  if ((s = enqueue_teacher(ctx, c)) != NE_OK || (s = enqueue_pack(ctx, c)) != NE_OK) return s;
-  const bool pair = rows >= 512;
-  const int tile_m = pair ? 2 * GEMM_BM : GEMM_BM;
-  // equal pieces of whole 256-id tiles, as few as the room for dz allows
-  const long long room = std::max<long long>(256, (long long)(kPieceBytes / 2) / rows64 / 256 * 256);
-  const int pieces = (int)((V + room - 1) / room);
-  const int piece = (int)up((V + pieces - 1) / pieces, 256);
-  for (int v0 = 0; v0 < V; v0 += piece) {
-    const int nv = std::min(piece, V - v0);
-    const int ldz = (int)up(nv, 64);
-    const __nv_bfloat16* w = (const __nv_bfloat16*)d.w + (long long)v0 * d.ldw;
-    CUtensorMap ta, tb, tc;
-    // dz = f(x . w^T)
-    if (!make_tmap(&ta, h->xp, rows64, D, D, GEMM_BM, 0) ||
-        !make_tmap(&tb, w, nv, D, d.ldw, pair ? 128 : 256, 0) ||
-        !make_tmap_out(&tc, h->dz, rows64, nv, ldz, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 32))
-      return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
-    EpiHeadDz::Params pz{};
-    pz.t = targets_of(h, c, true);
-    pz.lse = lse;
-    pz.grad = grad;
-    pz.c2 = d.scale / c.t * kLog2e;
-    pz.factor = c.t * d.scale;
-    pz.col0 = v0;
-    GemmShape sh = product_shape(rows, nv, D, tile_m, 256, h->count, 0, ctx->d_status);
-    if (pair) NE_LAUNCH((launch_product<256, EpiHeadDz, 0, 0, 2>(ta, tb, tc, sh, pz, sms, ctx->st)));
-    else NE_LAUNCH((launch_product<256, EpiHeadDz, 0, 0, 1>(ta, tb, tc, sh, pz, sms, ctx->st)));
-    if (g->dx) {   // dx (+)= dz . w
-      if (!make_tmap(&ta, h->dz, rows64, nv, ldz, GEMM_BM, 0) ||
-          !make_tmap_mn(&tb, w, D, nv, d.ldw) ||
-          !make_tmap_out(&tc, h->dx, rows64, D, D, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 32))
-        return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
-      sh = product_shape(rows, D, nv, tile_m, 256, h->count, 0, ctx->d_status);
-      const EpiF32S::Params ps{0};
-      const EpiResidS::Params pa{1.0f};
-      if (v0 == 0 && pair)
-        NE_LAUNCH((launch_product<256, EpiHeadF32, 0, 1, 2>(ta, tb, tc, sh, ps, sms, ctx->st)));
-      else if (v0 == 0)
-        NE_LAUNCH((launch_product<256, EpiHeadF32, 0, 1, 1>(ta, tb, tc, sh, ps, sms, ctx->st)));
-      else if (pair)
-        NE_LAUNCH((launch_product<256, EpiHeadAdd, 0, 1, 2>(ta, tb, tc, sh, pa, sms, ctx->st)));
-      else
-        NE_LAUNCH((launch_product<256, EpiHeadAdd, 0, 1, 1>(ta, tb, tc, sh, pa, sms, ctx->st)));
+  if ((s = enqueue_teacher(ctx, c)) != NE_OK ||
+      (s = enqueue_pack(ctx, c, plan.pieces + 1)) != NE_OK)
+    return s;
+  HeadDz dz{};
+  dz.t = targets_of(h, c, true);
+  dz.lse = lse;
+  dz.grad = grad;
+  dz.c2 = d.scale / c.t * kLog2e;
+  dz.factor = c.t * d.scale;
+  const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  HeadMaps maps;
+  bool ok = make_tmap(&maps.x_k, h->xp, rows64, D, D, GEMM_BM, 0) &&
+            make_tmap(&maps.w_k, d.w, V, D, d.ldw, HB_BN / plan.cg, 0) &&
+            make_tmap_mn(&maps.w_mn, d.w, D, V, d.ldw) &&
+            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, D) &&
+            make_tmap_out(&maps.dx_out, h->dx, plan.splits * rows64, D, D, f32, 4, 32);
+  HeadStep step{};
+  step.d_rows = h->count;
+  step.status = ctx->d_status;
+  step.rows64 = rows64;
+  step.dim = D;
+  step.dim_kb = (D + GEMM_BK - 1) / GEMM_BK;
+  step.dim_tiles = (D + HB_BN - 1) / HB_BN;
+  step.split_n = plan.split_n;
+  step.want_dx = g->dx != nullptr;
+  step.want_dw = g->dw != nullptr;
+  step.dw_f32 = g->dw_f32 != 0;
+  const int esz = g->dw_f32 ? 4 : 2;
+  const int ldz = plan.piece;
+  for (int p = 0; ok && p <= plan.pieces; ++p) {
+    step.counter = h->counters + p;
+    step.make0 = p * plan.piece;
+    step.make_n = p < plan.pieces ? std::min(plan.piece, V - step.make0) : 0;
+    step.use0 = (p - 1) * plan.piece;
+    step.use_n = p > 0 ? std::min(plan.piece, V - step.use0) : 0;
+    step.splits = (step.use_n + plan.split_n - 1) / plan.split_n;
+    step.dx_add = p > 1;
+    // a kind without units keeps another step's maps, which nothing reads
+    if (step.make_n)
+      ok = make_tmap_out(&maps.dz_out, h->dz[p & 1], rows64, step.make_n, ldz, bf, 2, 64);
+    if (ok && p > 0) {
+      const __nv_bfloat16* z = h->dz[(p - 1) & 1];
+      ok = make_tmap(&maps.dz_k, z, rows64, step.use_n, ldz, GEMM_BM, 0) &&
+           make_tmap_mn(&maps.dz_mn, z, step.use_n, rows64, ldz);
+      if (ok && g->dw)
+        ok = make_tmap_out(&maps.dw_out, (uint8_t*)g->dw + (long long)step.use0 * g->lddw * esz,
+                           step.use_n, D, g->lddw, g->dw_f32 ? f32 : bf, esz, 128 / esz);
+    } else if (ok) {
+      maps.dz_k = maps.dz_mn = maps.dw_out = maps.dz_out;
     }
-    if (g->dw) {   // dw = dz^T . x
-      const int esz = g->dw_f32 ? 4 : 2;
-      void* out = (uint8_t*)g->dw + (long long)v0 * g->lddw * esz;
-      const bool wide = nv >= 512;
-      if (!make_tmap_mn(&ta, h->dz, nv, rows64, ldz) || !make_tmap_mn(&tb, h->xp, D, rows64, D) ||
-          !make_tmap_out(&tc, out, nv, D, g->lddw,
-                         g->dw_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                         esz, 32))
-        return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
-      sh = product_shape(nv, D, rows, wide ? 256 : 128, 256, h->count, 1, ctx->d_status);
-      const EpiBF16S::Params pb{1.0f, 0};
-      const EpiResidS::Params pa{1.0f};
-      if (g->dw_f32 && wide)
-        NE_LAUNCH((launch_product<256, EpiHeadAdd, 1, 1, 2>(ta, tb, tc, sh, pa, sms, ctx->st)));
-      else if (g->dw_f32)
-        NE_LAUNCH((launch_product<256, EpiHeadAdd, 1, 1, 1>(ta, tb, tc, sh, pa, sms, ctx->st)));
-      else if (wide)
-        NE_LAUNCH((launch_product<256, EpiHeadBF16, 1, 1, 2>(ta, tb, tc, sh, pb, sms, ctx->st)));
-      else
-        NE_LAUNCH((launch_product<256, EpiHeadBF16, 1, 1, 1>(ta, tb, tc, sh, pb, sms, ctx->st)));
-    }
+    if (!ok) break;
+    if (plan.cg == 2) NE_LAUNCH(launch_step<2>(maps, step, dz, plan.clusters, ctx->st));
+    else NE_LAUNCH(launch_step<1>(maps, step, dz, plan.clusters, ctx->st));
   }
+  if (!ok) return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
   if (g->dx) {
     const dim3 grid((rows + 7) / 8);
+    const long long slab = (long long)rows64 * D;
+    const int slabs = (std::min(plan.piece, V) + plan.split_n - 1) / plan.split_n;
     if (g->dx_f32)
       NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
-                         rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx));
+                         slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx));
     else
       NE_LAUNCH(launch_k(head_dx_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->st,
-                         (const float*)h->dx, rows, D, (const int*)h->pos_of, (__nv_bfloat16*)g->dx,
-                         g->lddx));
+                         (const float*)h->dx, slabs, slab, rows, D, (const int*)h->pos_of,
+                         (__nv_bfloat16*)g->dx, g->lddx));
   }
   return NE_OK;
 }
@@ -818,8 +776,8 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   const size_t R = n.max_rows, R256 = up(R, 256), D = n.max_dim, V = n.max_vocab;
   const size_t K = std::max(n.max_topk, 1);
   // a piece is at least 256 ids wide, whatever the rows
-  n.dz_elems = std::max<size_t>(kPieceBytes / 2, up(R, 64) * 256);
-  n.dz_elems = std::min<size_t>(n.dz_elems, up(R, 64) * up(V, 256));
+  const size_t dz = std::min<size_t>(std::max<size_t>(kPieceBytes, up(R, 64) * HB_BN * 2),
+                                     up(R, 64) * up(V, HB_BN) * 2);
   // pairs: two a 256-id tile and row; up to one tile of rows, two a 64-id tile
   const size_t pairs = std::max(2 * ((V + 255) / 256) * R,
                                 2 * ((V + 63) / 64) * std::min<size_t>(R, GEMM_BM));
@@ -832,7 +790,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4),
                o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
                o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8),
-               o_xp = take(R256 * D * 2), o_dz = take(n.dz_elems * 2), o_dx = take(up(R, 64) * D * 4);
+               o_xp = take(R256 * D * 2), o_dz0 = take(dz), o_dz1 = take(dz),
+               o_dx = take(std::max(up(R, 64) * D * 4, kSlabBytes)),
+               o_counters = take((up(V, HB_BN) / HB_BN + 1) * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
   if (s != NE_OK) return s;
@@ -847,8 +807,10 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   n.zt = (float*)(b + o_zt);
   n.stats = (float2*)(b + o_stats);
   n.xp = (__nv_bfloat16*)(b + o_xp);
-  n.dz = (__nv_bfloat16*)(b + o_dz);
+  n.dz[0] = (__nv_bfloat16*)(b + o_dz0);
+  n.dz[1] = (__nv_bfloat16*)(b + o_dz1);
   n.dx = (float*)(b + o_dx);
+  n.counters = (int*)(b + o_counters);
   ctx->head = new HeadState(n);
   return NE_OK;
 }
