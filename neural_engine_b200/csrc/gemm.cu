@@ -383,8 +383,6 @@ cudaError_t gemm_run(const GemmCall& c, int* status, cudaStream_t st) {
   sh.kb_per_split = kb / splits;
   sh.status = status;
   sh.prefetch_a = c.prefetch_a;
-  sh.d_rows = nullptr;
-  sh.dyn_k = 0;
   // Raster groups when A outgrows a share of L2: M-fastest order re-reads all
   // of A for every wave of n-tiles once A no longer stays resident, so the
   // units run in groups of m-tiles whose A panels total ~48 MB (the wave's B

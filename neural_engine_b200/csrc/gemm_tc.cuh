@@ -48,26 +48,7 @@ struct GemmShape {
   int prefetch_a;       // A does not depend on the preceding kernel: its first
                         // tiles may be loaded before the PDL dependency wait
   int group_m;          // m-tiles per raster group (0: one group of all m-tiles)
-  const int* d_rows;    // device-sized products (EpiDyn): the number of rows that count
-  int dyn_k;            // they bound K (1) or M (0)
 };
-
-// Products whose row count the host does not know (rows packed on the device):
-// the tile and k-block counts follow *d_rows, rounded up to whole blocks of 64
-// rows, at least one.  The rows this adds are the caller's to neutralise, so
-// that a later product may reduce over whole blocks and a product of no rows
-// still writes its zeros.
-__device__ __forceinline__ GemmShape dyn_shape(GemmShape sh, int tile_m) {
-  const int blocks = max((*sh.d_rows + GEMM_BK - 1) / GEMM_BK, 1);
-  if (sh.dyn_k) {
-    sh.K = blocks * GEMM_BK;
-    sh.kb_per_split = blocks;
-  } else {
-    sh.M = blocks * GEMM_BK;
-    sh.m_tiles = (sh.M + tile_m - 1) / tile_m;
-  }
-  return sh;
-}
 
 // Work unit u -> (m tile, n tile, split).  Units run M-fastest inside groups
 // of group_m m-tiles: a wave of consecutive units covers a block of about
@@ -124,25 +105,6 @@ template <class E, class = void>
 struct EpiHasPrefetch { static constexpr bool value = false; };
 template <class E>
 struct EpiHasPrefetch<E, decltype(void(&E::prefetch))> { static constexpr bool value = true; };
-
-// A functor with kDyn takes its row count from device memory (dyn_shape).
-template <class E, class = void>
-struct EpiDyn { static constexpr bool value = false; };
-template <class E>
-struct EpiDyn<E, decltype(void(E::kDyn))> { static constexpr bool value = true; };
-
-// A functor with a `State` type keeps per-row values in registers over the
-// chunks of one work unit: begin(p, st, m, n_tile0, M) runs before the
-// accumulator is waited for, chunk() / stage() take the state, and
-// end(p, st, m, nt, half, M) runs after the warp's last chunk (half: which of
-// the two warps of the row this is).
-template <class E, class = void>
-struct EpiState { static constexpr bool value = false; struct type {}; };
-template <class E>
-struct EpiState<E, decltype(void(sizeof(typename E::State)))> {
-  static constexpr bool value = true;
-  using type = typename E::State;
-};
 
 // Vector (16-byte) accesses are used only where the row pointer allows them;
 // an output whose leading dimension leaves rows unaligned takes the scalar path.
@@ -730,9 +692,8 @@ template <int BN, class Epi, int AB_FMT, int A_MN = 0, int B_MN = 0, int CG = 1>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
-               const GemmShape sh_arg, const typename Epi::Params ep) {
+               const GemmShape sh, const typename Epi::Params ep) {
   using C = GemmCfg<BN, CG>;
-  constexpr bool DYN = EpiDyn<Epi>::value;
   constexpr bool PAIR = CG == 2;
   constexpr int TILE_M = GEMM_BM * CG;          // rows of A per work unit (both CTAs)
   static_assert(!PAIR || !EpiTransposed<Epi>::value, "pair tiles: row-major epilogues only");
@@ -762,6 +723,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const int units = sh.m_tiles * sh.n_tiles * sh.splits;
   // pair mode: both CTAs of a cluster walk the same units (one per cluster)
   const uint32_t crank = PAIR ? cluster_ctarank() : 0u;
   const int u_first = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
@@ -800,14 +762,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   if constexpr (PAIR) cluster_sync_all();   // the peer's barriers exist before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-
-  [[maybe_unused]] GemmShape sh_dyn;
-  if constexpr (DYN) {
-    pdl_wait();   // the row count is the preceding kernels' result
-    sh_dyn = dyn_shape(sh_arg, TILE_M);
-  }
-  const GemmShape& sh = DYN ? sh_dyn : sh_arg;
-  const int units = sh.m_tiles * sh.n_tiles * sh.splits;
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer
@@ -976,9 +930,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           Epi::prefetch(ep, mn * TILE_M + row0 + row_in_tile, nn * BN, BN, sh.M, sh.N);
         }
       }
-      [[maybe_unused]] typename EpiState<Epi>::type est;
-      if constexpr (EpiState<Epi>::value)
-        Epi::begin(ep, est, mt * TILE_M + row0 + row_in_tile, nt * BN, sh.M);
       // warp-uniform outcome: tcgen05.ld below is a warp-collective instruction
       const bool ready = mbar_wait(tfull_bar + 8 * acc, acc_phase, sh.status, abort_flag);
       if (!__all_sync(0xffffffffu, ready)) break;
@@ -1038,10 +989,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
         }
         if constexpr (STG == 0) {
-          if constexpr (EpiState<Epi>::value)
-            Epi::template chunk<CH>(ep, est, m, nt * BN + c, v, sh.M, sh.N);
-          else
-            Epi::template apply<CH>(ep, m, nt * BN + c, v, sp, sh.M, sh.N);
+          Epi::template apply<CH>(ep, m, nt * BN + c, v, sp, sh.M, sh.N);
         } else {
           // staged: 32 rows x kCols outputs -> swizzled box -> one TMA store / add
           static_assert(CH == 32, "staged epilogues work on 32-column chunks");
@@ -1059,8 +1007,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           } else if constexpr (EpiPre<Epi>::value) {
             Epi::template stage<CH>(ep, m, n0, v, o, sh.M, sh.N, pre_cur);
             pre_cur = pre_nxt;
-          } else if constexpr (EpiState<Epi>::value) {
-            Epi::template stage<CH>(ep, est, m, n0, v, o, sh.M, sh.N);
           } else {
             Epi::template stage<CH>(ep, m, n0, v, o, sh.M, sh.N);
           }
@@ -1104,7 +1050,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           }
         }
       }
-      if constexpr (EpiState<Epi>::value) Epi::end(ep, est, m, nt, chunk0 != 0, sh.M);
       tc_fence_before();
       if constexpr (PAIR) {
         // one arrival per warp, on the even CTA's barrier (the MMA issuer's)

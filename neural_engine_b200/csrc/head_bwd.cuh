@@ -61,6 +61,10 @@ __device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& 
   c.next = 0x7fffffff;
   if (c.row < 0) return;
   const int* ids = t.ids + c.row;
+  if (t.n == 1) {
+    c.next = *ids;
+    return;
+  }
   int lo = 0, hi = t.n;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;

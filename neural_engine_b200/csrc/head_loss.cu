@@ -32,6 +32,7 @@
 #include "gemm_tc.cuh"
 #include "gemm_tmap.h"
 #include "head_bwd.cuh"
+#include "head_fwd.cuh"
 #include "ne_ctx.h"
 #include "ne_internal.h"
 #include "ne_launch.cuh"
@@ -70,78 +71,6 @@ constexpr size_t kPieceBytes = 128u << 20;
 constexpr size_t kSlabBytes = 64u << 20;
 
 inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
-
-// ------------------------------------------------------------------ forward epilogue
-// Forward: a thread owns one row of the tile and half of its column chunks.
-// It keeps the running maximum m and sum s of exp2(c2 * acc - m), c2 = scale /
-// (T ln 2), in fp32 registers, and writes one pair a tile: 8 bytes for 128
-// logits.
-struct EpiHeadLse {
-  struct Params {
-    HeadTargets t;
-    float2* stats;
-    long long part_stride, row_stride;
-    float* zt;
-    float c2;
-  };
-  struct State {
-    float mx, sum;
-    TargetCursor c;
-  };
-  __device__ static void begin(const Params& p, State& st, int m, int col0, int M) {
-    st.mx = kLowest;
-    st.sum = 0.f;
-    cursor_seek(p.t, st.c, m, M, col0);
-  }
-  template <int CH>
-  __device__ static void chunk(const Params& p, State& st, int, int n0, const float (&v)[CH], int,
-                               int N) {
-    if (st.c.row < 0 || n0 >= N) return;
-    float top = kLowest;
-    if (n0 + CH <= N) {
-#pragma unroll
-      for (int j = 0; j < CH; ++j) top = fmaxf(top, v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-        if (n0 + j < N) top = fmaxf(top, v[j]);
-    }
-    const float mx = fmaxf(st.mx, top * p.c2);
-    float s0 = st.sum * ex2_fast(st.mx - mx), s1 = 0.f;
-    if (n0 + CH <= N) {
-#pragma unroll
-      for (int j = 0; j < CH; j += 2) {
-        s0 += ex2_fast(fmaf(v[j], p.c2, -mx));
-        s1 += ex2_fast(fmaf(v[j + 1], p.c2, -mx));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-        if (n0 + j < N) s0 += ex2_fast(fmaf(v[j], p.c2, -mx));
-    }
-    st.mx = mx;
-    st.sum = s0 + s1;
-    while (st.c.next < n0 + CH) {
-      if (st.c.next >= n0) {
-        const int j = st.c.next - n0;
-        float z = 0.f;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (i == j) z = v[i];
-        p.zt[st.c.at * p.t.ld + st.c.row] = z * p.c2;
-      }
-      cursor_step(p.t, st.c);
-    }
-  }
-  __device__ static void end(const Params& p, State& st, int m, int nt, int half, int) {
-    if (st.c.row >= 0)
-      p.stats[(2 * nt + half) * p.part_stride + m * p.row_stride] = make_float2(st.mx, st.sum);
-  }
-};
-// the same over packed rows, whose number stands in device memory
-struct EpiHeadLseDyn : EpiHeadLse {
-  static constexpr int kDyn = 1;
-};
 
 // ------------------------------------------------------------------ rows
 __device__ __forceinline__ bool row_counts(const int32_t* target, const int* keep, int i, int vocab) {
@@ -385,7 +314,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
 }
 
 // dx of the rows as the caller laid them out, the slabs added in their order;
-// zeros where a row was left out.
+// zeros where a row was left out.  A thread takes four columns.
 template <class T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int slabs,
                                                       long long slab, int rows, int dim,
@@ -393,71 +322,76 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
                                                       long long ld) {
   pdl_trigger();
   pdl_wait();
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= rows) return;
+  const int quads = dim / 4;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= (long long)rows * quads) return;
+  const int i = (int)(at / quads), k = (int)(at - (long long)i * quads);
   const int pos = pos_of[i];
-  const float4* src = reinterpret_cast<const float4*>(acc + (long long)(pos < 0 ? 0 : pos) * dim);
-  T* dst = dx + (long long)i * ld;
-  for (int k = threadIdx.x & 31; k < dim / 4; k += 32) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (pos >= 0) {
-      v = src[k];
-      for (int u = 1; u < slabs; ++u) {
-        const float4 q = src[k + u * (slab / 4)];
-        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-      }
-    }
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(dst)[k] = v;
-    } else {
-      uint2 o;
-      *reinterpret_cast<__nv_bfloat162*>(&o.x) = __floats2bfloat162_rn(v.x, v.y);
-      *reinterpret_cast<__nv_bfloat162*>(&o.y) = __floats2bfloat162_rn(v.z, v.w);
-      reinterpret_cast<uint2*>(dst)[k] = o;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (pos >= 0) {
+    const float4* src = reinterpret_cast<const float4*>(acc + (long long)pos * dim) + k;
+#pragma unroll 8
+    for (int u = 0; u < slabs; ++u) {
+      const float4 q = src[u * (slab / 4)];
+      v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
     }
   }
-}
-
-// ------------------------------------------------------------------ products
-template <int BN, class Epi, int AMN, int BMN, int CG>
-cudaError_t launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
-                           const GemmShape& sh, const typename Epi::Params& p, int num_sms,
-                           cudaStream_t st) {
-  using C = GemmCfg<BN, CG>;
-  constexpr int smem = EpiStage<Epi>::value ? C::SMEM_BYTES_STAGED : C::SMEM_BYTES;
-  auto kern = gemm_tc_kernel<BN, Epi, 1, AMN, BMN, CG>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  const long long units = (long long)sh.m_tiles * sh.n_tiles;
-  CUtensorMap td{};
-  if constexpr (CG == 2) {
-    const int grid = (int)(2 * std::min<long long>(units, num_sms / 2));
-    return launch_k_cluster(kern, dim3(grid), dim3(GEMM_THREADS), (size_t)smem, st, 2u, ta, tb, tc,
-                            td, sh, p);
+  T* dst = dx + (long long)i * ld + 4 * k;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(dst) = v;
   } else {
-    const int grid = (int)std::min<long long>(units, num_sms);
-    return launch_k(kern, dim3(grid), dim3(GEMM_THREADS), (size_t)smem, st, ta, tb, tc, td, sh, p);
+    uint2 o;
+    *reinterpret_cast<__nv_bfloat162*>(&o.x) = __floats2bfloat162_rn(v.x, v.y);
+    *reinterpret_cast<__nv_bfloat162*>(&o.y) = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(dst) = o;
   }
 }
 
-GemmShape product_shape(int M, int N, int K, int tile_m, int bn, const int* d_rows, int dyn_k,
-                        int* status) {
-  GemmShape sh{};
-  sh.M = M;
-  sh.N = N;
-  sh.K = K;
-  sh.m_tiles = (M + tile_m - 1) / tile_m;
-  sh.n_tiles = (N + bn - 1) / bn;
-  sh.splits = 1;
-  sh.kb_per_split = (K + GEMM_BK - 1) / GEMM_BK;
-  sh.status = status;
-  sh.d_rows = d_rows;
-  sh.dyn_k = dyn_k;
-  // as gemm_run: m-tiles whose A panels stay in L2 while a wave of tiles reuses them
-  const long long panel = (long long)tile_m * K * 2, budget = 48ll << 20;
-  if (sh.n_tiles > 1 && panel * sh.m_tiles > budget)
-    sh.group_m = (int)std::max<long long>(1, budget / panel);
-  return sh;
+// ------------------------------------------------------------------ host
+// How the forward pass tiles rows and ids.
+struct LsePlan {
+  int cg, clusters;           // CTAs a tile, tiles at once
+  bool packed, one_row_tile;
+  int bn, a_rows, stages;
+  size_t smem;
+};
+
+LsePlan lse_plan(int rows, int dim, int vocab, int num_sms) {
+  LsePlan p;
+  p.cg = rows > GEMM_BM ? 2 : 1;
+  p.one_row_tile = rows <= GEMM_BM * p.cg;
+  p.packed = !p.one_row_tile;   // within one tile of rows packing saves nothing
+  p.clusters = num_sms / p.cg;
+  const int tile_m = GEMM_BM * p.cg, m_tiles = (rows + tile_m - 1) / tile_m;
+  const double dim_kb = (dim + GEMM_BK - 1) / GEMM_BK;
+  // ids a tile: what the busiest SM has to do, in ids -- whole waves of tiles,
+  // about 700 cycles of hand-over a tile (a k-block takes 2 an id), and the last
+  // tile's epilogue, which nothing hides
+  double best = 0;
+  p.bn = 256;
+  for (int bn = 256; bn >= (p.cg == 2 ? 192 : 96); bn -= 16 * p.cg) {
+    const long long units = (long long)m_tiles * ((vocab + bn - 1) / bn);
+    const double waves = (double)((units + p.clusters - 1) / p.clusters);
+    const double cost = waves * (bn + 350 / dim_kb) + 6 * bn / dim_kb;
+    if (bn == 256 || cost < best) {
+      best = cost;
+      p.bn = bn;
+    }
+  }
+  p.a_rows = p.cg == 2 ? GEMM_BM : (int)up(rows, 8);
+  const int a = p.a_rows * 128, b = p.bn / p.cg * 128;
+  // 1 KB each for alignment and barriers; an MMA reads 128 rows of x
+  const int fixed = 2048 + GEMM_BM * 128 - a;
+  p.stages = std::min(HF_MAX_STAGES, (227 * 1024 - fixed) / (a + b));
+  p.smem = (size_t)fixed + (size_t)p.stages * (a + b);
+  return p;
+}
+
+// m-tiles whose panels of x stay in L2 while a wave of tiles reuses them (as gemm_run)
+int raster_group(int rows, int dim, int tile_m) {
+  const long long panel = (long long)tile_m * dim * 2, budget = 48ll << 20;
+  const long long m_tiles = (rows + tile_m - 1) / tile_m;
+  return panel * m_tiles > budget ? (int)std::max<long long>(1, budget / panel) : 0;
 }
 
 // What a call works on, after its arguments were checked.
@@ -530,37 +464,55 @@ HeadTargets targets_of(const HeadState* h, const HeadCall& c, bool packed) {
   return t;
 }
 
+template <int CG>
+cudaError_t launch_lse(const CUtensorMap& x, const CUtensorMap& w, const HeadLse& p,
+                       const LsePlan& plan, long long units, cudaStream_t st) {
+  auto kern = head_lse_kernel<CG>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan.smem);
+  if (e != cudaSuccess) return e;
+  const int grid = CG * (int)std::min<long long>(units, plan.clusters);
+  if constexpr (CG == 2)
+    return launch_k_cluster(kern, dim3(grid), dim3(HB_THREADS), plan.smem, st, 2u, x, w, p);
+  else
+    return launch_k(kern, dim3(grid), dim3(HB_THREADS), plan.smem, st, x, w, p);
+}
+
 ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) {
   HeadState* h = ctx->head;
   const ne_head_desc& d = *c.d;
-  const int rows = d.rows, V = d.vocab, D = d.dim, sms = ctx->num_sms;
+  const int rows = d.rows, V = d.vocab, D = d.dim;
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK) return s;
-  // up to one tile of rows, nothing is saved by packing
-  const bool packed = rows > GEMM_BM;
-  const bool pair = rows >= 512;
-  const int bn = packed ? 256 : 64;
-  if (packed && (s = enqueue_pack(ctx, c, 0)) != NE_OK) return s;
-  EpiHeadLse::Params p{};
-  p.t = targets_of(h, c, packed);
+  const LsePlan plan = lse_plan(rows, D, V, ctx->num_sms);
+  if (plan.packed && (s = enqueue_pack(ctx, c, 0)) != NE_OK) return s;
+  const int tile_m = GEMM_BM * plan.cg;
+  const int n_tiles = (V + plan.bn - 1) / plan.bn;
+  const long long units = (long long)((rows + tile_m - 1) / tile_m) * n_tiles;
+  const int parts = 2 * (plan.one_row_tile ? (int)std::min<long long>(units, plan.clusters) : n_tiles);
+  HeadLse p{};
+  p.t = targets_of(h, c, plan.packed);
+  p.d_rows = plan.packed ? h->count : nullptr;
+  p.status = ctx->d_status;
   p.stats = h->stats;
-  const int parts = 2 * ((V + bn - 1) / bn);
-  p.part_stride = packed ? rows : 1;
-  p.row_stride = packed ? 1 : parts;
+  p.part_stride = plan.one_row_tile ? 1 : rows;
+  p.row_stride = plan.one_row_tile ? parts : 1;
   p.zt = h->zt;
   p.c2 = d.scale / c.t * kLog2e;
-  const int tile_m = pair ? 2 * GEMM_BM : GEMM_BM;
-  const GemmShape sh = product_shape(rows, V, D, tile_m, bn, h->count, 0, ctx->d_status);
-  CUtensorMap ta, tb, tc{};
-  if (!make_tmap(&ta, packed ? h->xp : d.x, rows, D, packed ? D : d.ldx, GEMM_BM, 0) ||
-      !make_tmap(&tb, d.w, V, D, d.ldw, pair ? bn / 2 : bn, 0))
+  p.rows = rows;
+  p.vocab = V;
+  p.dim_kb = (D + GEMM_BK - 1) / GEMM_BK;
+  p.bn = plan.bn;
+  p.n_tiles = n_tiles;
+  p.group_m = raster_group(rows, D, tile_m);
+  p.a_rows = plan.a_rows;
+  p.stages = plan.stages;
+  p.one_row_tile = plan.one_row_tile;
+  CUtensorMap x, w;
+  if (!make_tmap(&x, plan.packed ? h->xp : d.x, rows, D, plan.packed ? D : d.ldx, plan.a_rows, 0) ||
+      !make_tmap(&w, d.w, V, D, d.ldw, plan.bn / plan.cg, 0))
     return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
-  if (pair)
-    NE_LAUNCH((launch_product<256, EpiHeadLseDyn, 0, 0, 2>(ta, tb, tc, sh, p, sms, ctx->st)));
-  else if (packed)
-    NE_LAUNCH((launch_product<256, EpiHeadLseDyn, 0, 0, 1>(ta, tb, tc, sh, p, sms, ctx->st)));
-  else
-    NE_LAUNCH((launch_product<64, EpiHeadLse, 0, 0, 1>(ta, tb, tc, sh, p, sms, ctx->st)));
+  if (plan.cg == 2) NE_LAUNCH(launch_lse<2>(x, w, p, plan, units, ctx->st));
+  else NE_LAUNCH(launch_lse<1>(x, w, p, plan, units, ctx->st));
   HeadJoin j{};
   j.stats = h->stats;
   j.part_stride = p.part_stride;
@@ -569,7 +521,7 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   j.rows = rows;
   j.vocab = V;
   j.n = c.n;
-  j.pos_of = packed ? h->pos_of : nullptr;
+  j.pos_of = plan.packed ? h->pos_of : nullptr;
   j.target = c.target;
   j.keep = c.teacher ? h->keep : nullptr;
   j.ids = h->ids;
@@ -580,7 +532,7 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   j.loss = loss;
   j.lse = lse;
   j.status = ctx->d_status;
-  if (packed)
+  if (plan.packed)
     NE_LAUNCH(launch_k(head_join_kernel<32>, dim3((rows + 31) / 32), dim3(256), 0, ctx->st, j));
   else
     NE_LAUNCH(launch_k(head_join_kernel<1>, dim3(rows), dim3(256), 0, ctx->st, j));
@@ -697,7 +649,7 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   }
   if (!ok) return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
   if (g->dx) {
-    const dim3 grid((rows + 7) / 8);
+    const dim3 grid((unsigned)(((long long)rows * (D / 4) + 255) / 256));
     const long long slab = (long long)rows64 * D;
     const int slabs = (std::min(plan.piece, V) + plan.split_n - 1) / plan.split_n;
     if (g->dx_f32)
@@ -778,9 +730,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   // a piece is at least 256 ids wide, whatever the rows
   const size_t dz = std::min<size_t>(std::max<size_t>(kPieceBytes, up(R, 64) * HB_BN * 2),
                                      up(R, 64) * up(V, HB_BN) * 2);
-  // pairs: two a 256-id tile and row; up to one tile of rows, two a 64-id tile
-  const size_t pairs = std::max(2 * ((V + 255) / 256) * R,
-                                2 * ((V + 63) / 64) * std::min<size_t>(R, GEMM_BM));
+  // pairs of a row: two a tile of at least 192 ids, or two a CTA where there is
+  // one tile of rows
+  const size_t pairs = std::max(2 * ((V + 191) / 192) * R, (size_t)2 * ctx->num_sms * 2 * GEMM_BM);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
