@@ -27,6 +27,18 @@ namespace ne {
 constexpr int HB_BN = 256;
 constexpr int HB_SLOTS = 4;
 constexpr int HB_THREADS = GEMM_THREADS + 32;   // warps: A, MMA, 8 x epilogue, B
+constexpr int HB_BOX = 4096;                    // 32 rows of 128 bytes
+constexpr int HB_TAB = 256;                     // ids per entry of a row's index
+
+template <int CG>
+struct HeadCfg {
+  static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + HB_BN / CG * GEMM_BK * 2;
+  static constexpr int STAGES = CG == 2 ? 5 : 3;
+  // ring, barriers, two boxes per epilogue warp, alignment
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 2048 + GEMM_EPI_WARPS * 2 * HB_BOX;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
 
 struct HeadStep {
   const int* d_rows;        // packed rows
@@ -41,50 +53,49 @@ struct HeadStep {
   int want_dx, want_dw, dx_add, dw_f32;
 };
 
-// The sparse targets of a row: sorted ids, [entry][row].
+// The sparse targets of the rows: sorted ids, [entry][row], INT_MAX behind the
+// last.
 struct HeadTargets {
   const int* ids;
-  const float* prob;     // backward: the probability of each id (NULL: 1)
-  const int* row_of;     // NULL: rows are not packed
-  long long ld;          // between entries
-  int n;                 // entries a row
+  const float* prob;           // the probability of each id (NULL: 1)
+  const int* row_of;           // packed row -> row of the arrays (NULL: the same)
+  const unsigned short* tab;   // [row][tab_ld]: how many ids are below 256 t (NULL: one entry a row)
+  long long ld;                // between entries
+  int tab_ld;
+  int n;                       // entries a row
 };
 
 struct TargetCursor {
-  int row, at, next;     // row (-1: none), entry, its id
+  int row, at, next;     // row of the arrays (-1: none), entry, its id
 };
 
-__device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& c, int m, int M,
+// The first entry of row m with an id of at least col0.  Few entries lie
+// between a multiple of 256 and col0, so they are stepped over; a search of the
+// whole row would be a chain of log2 n loads, 600 cycles each.
+__device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& c, int m, int rows,
                                             int col0) {
-  c.row = m < M ? (t.row_of ? t.row_of[m] : m) : -1;
+  c.row = m < rows ? (t.row_of ? t.row_of[m] : m) : -1;
   c.at = 0;
   c.next = 0x7fffffff;
   if (c.row < 0) return;
-  const int* ids = t.ids + c.row;
-  if (t.n == 1) {
-    c.next = *ids;
-    return;
+  if (t.tab) c.at = t.tab[(long long)c.row * t.tab_ld + col0 / HB_TAB];
+  while (c.at < t.n) {
+    c.next = t.ids[c.at * t.ld + c.row];
+    if (c.next >= col0) return;
+    ++c.at;
   }
-  int lo = 0, hi = t.n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ids[mid * t.ld] < col0) lo = mid + 1;
-    else hi = mid;
-  }
-  c.at = lo;
-  if (lo < t.n) c.next = ids[lo * t.ld];
+  c.next = 0x7fffffff;
 }
 __device__ __forceinline__ void cursor_step(const HeadTargets& t, TargetCursor& c) {
   ++c.at;
   c.next = c.at < t.n ? t.ids[c.at * t.ld + c.row] : 0x7fffffff;
 }
 
-// What turns logits into dz = a (exp2(c2 acc - lse2) - p), a = g T scale.
+// What turns logits into dz = a (2^(c2 acc - lse log2 e) - p), a = g T scale.
 struct HeadDz {
   HeadTargets t;
-  const float* lse;
-  const float* grad;    // NULL: 1
-  float c2, factor;     // scale / (T ln 2), T * scale
+  const float2* coef;   // packed rows: a, log2|a| - lse log2 e
+  float c2;             // scale / (T ln 2)
 };
 
 struct HeadMaps {
@@ -100,7 +111,12 @@ enum HeadKind : int { HK_DX = 0, HK_DW = 1, HK_DZ = 2 };
 
 struct HeadUnit {
   int kind, mt, nt, split, kb0, kb;
+  int n;   // columns: 256, or what is left of them in whole 32s
 };
+
+__device__ __forceinline__ int unit_cols(int cols, int nt) {
+  return min(HB_BN, (cols - nt * HB_BN + 31) & ~31);
+}
 
 // unit u of the step, dx first (the longest), dz last
 __device__ __forceinline__ bool head_unit(const HeadStep& s, int rows_blocks, int m_tiles, int tile_m,
@@ -117,6 +133,7 @@ __device__ __forceinline__ bool head_unit(const HeadStep& s, int rows_blocks, in
     o.kb0 = o.split * (s.split_n / GEMM_BK);
     const int left = s.use_n - o.split * s.split_n;
     o.kb = (min(left, s.split_n) + GEMM_BK - 1) / GEMM_BK;
+    o.n = unit_cols(s.dim, o.nt);
     return true;
   }
   u -= n_dx;
@@ -127,6 +144,7 @@ __device__ __forceinline__ bool head_unit(const HeadStep& s, int rows_blocks, in
     o.nt = u % s.dim_tiles;
     o.mt = u / s.dim_tiles;
     o.kb = rows_blocks;
+    o.n = unit_cols(s.dim, o.nt);
     return true;
   }
   u -= n_dw;
@@ -135,6 +153,7 @@ __device__ __forceinline__ bool head_unit(const HeadStep& s, int rows_blocks, in
     o.mt = u % m_tiles;
     o.nt = u / m_tiles;
     o.kb = s.dim_kb;
+    o.n = unit_cols(s.make_n, o.nt);
     return true;
   }
   return false;
@@ -203,10 +222,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 template <int CG>
 __global__ void __launch_bounds__(HB_THREADS, 1)
 head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const HeadDz dzp) {
-  using C = GemmCfg<HB_BN, CG>;
+  using C = HeadCfg<CG>;
   constexpr bool PAIR = CG == 2;
   constexpr int TILE_M = GEMM_BM * CG;
   constexpr int STAGES = C::STAGES;
+  constexpr uint32_t TMEM_COLS = 2 * HB_BN;
   constexpr uint32_t MN_BOX = 64 * GEMM_BK * 2;
   constexpr int B_ROWS = HB_BN / CG;
   // readers of a slot: the MMA thread, B's producer and 8 epilogue warps, and the
@@ -254,10 +274,10 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
   }
   if (warp == 1) {
     if constexpr (PAIR) {
-      tmem_alloc_pair(smem_u32(tmem_slot), C::TMEM_COLS);
+      tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
       tmem_relinquish_pair();
     } else {
-      tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+      tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
       tmem_relinquish();
     }
   }
@@ -269,7 +289,8 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
   // whole blocks of 64 rows, at least one (its rows are zeros)
-  const int blocks = max((*sp.d_rows + GEMM_BK - 1) / GEMM_BK, 1);
+  const int count = *sp.d_rows;
+  const int blocks = max((count + GEMM_BK - 1) / GEMM_BK, 1);
   const int M = blocks * GEMM_BK;
   const int m_tiles = (M + TILE_M - 1) / TILE_M;
 
@@ -325,7 +346,7 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
                  : (w.kind == HK_DZ ? &maps.w_k : w.kind == HK_DX ? &maps.w_mn : &maps.x_mn);
         // first row (K-major) or column (MN-major) of the tile, and where K starts
         const int first = is_a ? w.mt * TILE_M + (int)crank * GEMM_BM
-                               : w.nt * HB_BN + (int)crank * B_ROWS + (w.kind == HK_DZ ? sp.make0 : 0);
+                               : w.nt * HB_BN + (int)crank * (w.n / CG) + (w.kind == HK_DZ ? sp.make0 : 0);
         int k0 = w.kb0 * GEMM_BK + (!is_a && w.kind == HK_DX ? sp.use0 : 0);
         for (int k = 0; k < w.kb; ++k, k0 += GEMM_BK) {
           const uint32_t bar = full_to + 8 * stage;
@@ -376,7 +397,7 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * HB_BN;
         const int a_mn = w.kind == HK_DW, b_mn = w.kind != HK_DZ;
-        const uint32_t idesc = umma_idesc_f16(TILE_M, HB_BN, 1) | ((uint32_t)a_mn << 15) |
+        const uint32_t idesc = umma_idesc_f16(TILE_M, w.n, 1) | ((uint32_t)a_mn << 15) |
                                ((uint32_t)b_mn << 16);
         const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
         bool ok = true;
@@ -413,7 +434,7 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
     // ------------------------------------------------ epilogue (warps 2..9)
     const int quarter = warp & 3;
     const int half = (warp - 2) >> 2;
-    const uint32_t sbuf = base + STAGES * C::STAGE_BYTES + 1024 + (warp - 2) * GEMM_STAGE_SLOT;
+    const uint32_t sbuf = base + STAGES * C::STAGE_BYTES + 1024 + (warp - 2) * 2 * HB_BOX;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int it = 0;; ++it) {
@@ -432,14 +453,15 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
       float mag = 0.f, shift = 0.f;
       uint32_t keep = 0u, sign = 0u;
       if (w.kind == HK_DZ) {
-        cursor_seek(dzp.t, cur, y0 + lane, M, sp.make0 + n_tile + 128 * half);
-        if (cur.row >= 0) {
-          const float a = (dzp.grad ? dzp.grad[cur.row] : 1.0f) * dzp.factor;
-          mag = fabsf(a);
-          shift = __log2f(mag) - dzp.lse[cur.row] * 1.4426950408889634f;
+        const int m = y0 + lane;
+        if (m < count) {
+          const float2 co = dzp.coef[m];
+          mag = fabsf(co.x);
+          shift = co.y;
           keep = 0xffffffffu;
-          sign = a < 0.f ? 0x80008000u : 0u;
+          sign = co.x < 0.f ? 0x80008000u : 0u;
         }
+        cursor_seek(dzp.t, cur, m, count, sp.make0 + n_tile + 128 * half);
       }
       const bool ready = mbar_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag);
       if (!__all_sync(0xffffffffu, ready)) break;
@@ -450,58 +472,69 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
       const int cols_end = w.kind == HK_DZ ? sp.make_n : sp.dim;
       const CUtensorMap* out = w.kind == HK_DZ ? &maps.dz_out
                                : w.kind == HK_DW ? &maps.dw_out : &maps.dx_out;
-      // a warp owns half of the tile's columns and sends 128-byte rows: 64
-      // columns of bf16 or 32 of fp32 at a time
+      // a warp owns half of the tile's columns and sends boxes of 128-byte rows,
+      // 64 columns of bf16 or 32 of fp32, two at a time: the fence between the
+      // writes of a box and its store costs about 600 cycles
       const int step = b16 ? 64 : 32;
       const bool add = w.kind == HK_DX ? sp.dx_add : w.kind == HK_DW && sp.dw_f32;
       const int y = w.kind == HK_DX ? w.split * sp.rows64 + y0 : y0;
 #pragma unroll 1
-      for (int c = 128 * half; c < 128 * half + 128; c += step) {
-        const int n0 = n_tile + c;
-        uint32_t o[32];
-        if (b16) {
+      for (int c0 = 128 * half; c0 < 128 * half + 128; c0 += 2 * step) {
+        if (n_tile + c0 >= cols_end) break;
+        if (lane == 0) bulk_wait_read_all();   // the previous boxes have left
+        __syncwarp();
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b) {
+          const int c = c0 + b * step, n0 = n_tile + c;
+          if (n0 >= cols_end) break;
+          uint32_t o[32];
+          if (b16) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v[32];
-            tmem_ld32(t_row + c + 32 * h, v);
+            for (int h = 0; h < 2; ++h) {
+              float v[32];
+              tmem_ld32(t_row + c + 32 * h, v);
+              if (w.kind == HK_DZ) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
+                const int col = sp.make0 + n0 + 32 * h;
+                while (cur.next < col + 32) {
+                  if (cur.next >= col) {
+                    const int j = cur.next - col;
+                    const float q = dzp.t.prob ? dzp.t.prob[cur.at * dzp.t.ld + cur.row] : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                      if (i == j) v[i] -= mag * q;
+                  }
+                  cursor_step(dzp.t, cur);
+                }
+              }
+              // rounded once to bf16: dz is the operand of two tensor-core
+              // products, dw the caller's type
+              pack_bf16(v, o + 16 * h);
+            }
             if (w.kind == HK_DZ) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
-              const int col = sp.make0 + n0 + 32 * h;
-              while (cur.next < col + 32) {
-                if (cur.next >= col) {
-                  const int j = cur.next - col;
-                  const float q = dzp.t.prob ? dzp.t.prob[cur.at * dzp.t.ld + cur.row] : 1.0f;
-#pragma unroll
-                  for (int i = 0; i < 32; ++i)
-                    if (i == j) v[i] -= mag * q;
-                }
-                cursor_step(dzp.t, cur);
-              }
+              for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
             }
-            // rounded once to bf16: dz is the operand of two tensor-core
-            // products, dw the caller's type
-            pack_bf16(v, o + 16 * h);
-          }
-          if (w.kind == HK_DZ) {
+          } else {
+            float v[32];
+            tmem_ld32(t_row + c, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
           }
-        } else {
-          float v[32];
-          tmem_ld32(t_row + c, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
+          stage_words(sbuf + b * HB_BOX, lane, o);
         }
-        if (lane == 0) bulk_wait_read_all();   // the previous box has left the slot
-        __syncwarp();
-        stage_words(sbuf, lane, o);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (rows_in && n0 < cols_end) {
-            if (add) tma_reduce_add_2d(out, sbuf, n0, y);
-            else tma_store_2d(out, sbuf, n0, y);
+          if (rows_in) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int n0 = n_tile + c0 + b * step;
+              if (n0 >= cols_end) break;
+              if (add) tma_reduce_add_2d(out, sbuf + b * HB_BOX, n0, y);
+              else tma_store_2d(out, sbuf + b * HB_BOX, n0, y);
+            }
           }
           bulk_commit_group();
         }
@@ -522,8 +555,8 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
   if constexpr (PAIR) cluster_sync_all();
   tc_fence_after();
   if (warp == 1) {
-    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
-    else tmem_dealloc(tmem_base, C::TMEM_COLS);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 

@@ -45,15 +45,18 @@ struct HeadState {
   int max_dim = 0, max_topk = 0;
   void* pool = nullptr;
   int* count = nullptr;           // rows that count
-  int* row_of = nullptr;          // packed row -> row, -1 up to the next 64
+  int* row_of = nullptr;          // packed row -> row
   int* pos_of = nullptr;          // row -> packed row, -1 where left out
   int* keep = nullptr;            // distillation: the row has an entry
+  int* target = nullptr;          // cross entropy: targets of the packed rows
+  float2* coef = nullptr;         // packed rows: a, log2|a| - lse log2 e
   int* ids = nullptr;             // [topk][rows] sorted, INT_MAX behind the last
+  unsigned short* tab = nullptr;  // [rows][ids / 256 + 1] entries below each multiple of 256
   float* prob = nullptr;          // [topk][rows]
   float* neg_entropy = nullptr;   // [rows] sum p log p
   float* zt = nullptr;            // [topk][rows] target logits, log2 units
   float2* stats = nullptr;        // (max, sum exp2) of each row and half tile
-  __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim] packed x
+  __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim up to 64] packed x
   __nv_bfloat16* dz[2] = {};      // the pieces of dz that are made and used
   float* dx = nullptr;            // [splits][rows up to 64][dim] sums over the pieces
   int* counters = nullptr;        // work units drawn, one per backward step
@@ -79,21 +82,44 @@ __device__ __forceinline__ bool row_counts(const int32_t* target, const int* kee
   return t >= 0 && t < vocab;
 }
 
-// Moves the rows that count together, in order.  A block takes 32 rows; how
+// Moves the rows that count together, in order.  A block takes 8 to 32 rows; how
 // many count before them it counts itself (the targets stay in L2: 4 bytes a
 // row, once per block), so there is no scan to wait for.
 constexpr int PACK_ROWS = 32;
-__global__ void __launch_bounds__(256) head_pack_kernel(
-    const __nv_bfloat16* __restrict__ x, long long ldx, int rows, int dim,
-    const int32_t* __restrict__ target, const int* __restrict__ keep, int vocab, int* row_of,
-    int* pos_of, int* count, __nv_bfloat16* xp, int* counters, int n_counters, int* status) {
+int pack_rows(int rows) { return rows <= 2048 ? 8 : rows <= 8192 ? 16 : PACK_ROWS; }
+struct HeadPack {
+  const __nv_bfloat16* x;
+  long long ldx;
+  int rows, dim, vocab;
+  int per;                  // rows a block
+  const int32_t* target;    // cross entropy
+  const int* keep;          // distillation
+  int* row_of;
+  int* pos_of;
+  int* count;
+  int* target_p;
+  __nv_bfloat16* xp;        // rows of whole 128-byte lines: what a box of 64 columns reads
+  long long ldp;
+  // backward
+  const float* lse;
+  const float* grad;        // NULL: ones
+  float factor;             // T * scale
+  float2* coef;             // NULL: forward
+  int* counters;
+  int n_counters;
+  int* status;
+};
+__global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
   pdl_trigger();
   pdl_wait();
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
+    for (int i = threadIdx.x; i < p.n_counters; i += 256) p.counters[i] = 0;
+  const int32_t* target = p.target;
+  const int* keep = p.keep;
+  const int rows = p.rows, vocab = p.vocab, per = p.per;
   __shared__ int before, base_s;
   __shared__ unsigned mask_s;
-  const int first = blockIdx.x * PACK_ROWS;
+  const int first = blockIdx.x * per;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) before = 0;
   __syncthreads();
@@ -104,12 +130,20 @@ __global__ void __launch_bounds__(256) head_pack_kernel(
   __syncthreads();
   if (warp == 0) {
     const int i = first + lane;
-    const bool on = i < rows && row_counts(target, keep, i, vocab);
-    if (!keep && i < rows && target[i] >= vocab) atomicExch(status, DEV_ERR_BOUNDS);
+    const bool mine = lane < per && i < rows;
+    const bool on = mine && row_counts(target, keep, i, vocab);
+    if (!keep && mine && target[i] >= vocab) atomicExch(p.status, DEV_ERR_BOUNDS);
     const unsigned mask = __ballot_sync(0xffffffffu, on);
     const int pos = before + __popc(mask & ((1u << lane) - 1));
-    if (i < rows) pos_of[i] = on ? pos : -1;
-    if (on) row_of[pos] = i;
+    if (mine) p.pos_of[i] = on ? pos : -1;
+    if (on) {
+      p.row_of[pos] = i;
+      if (target) p.target_p[pos] = target[i];
+      if (p.coef) {
+        const float a = (p.grad ? p.grad[i] : 1.0f) * p.factor;
+        p.coef[pos] = make_float2(a, log2f(fabsf(a)) - p.lse[i] * kLog2e);
+      }
+    }
     if (lane == 0) {
       mask_s = mask;
       base_s = before;
@@ -117,37 +151,42 @@ __global__ void __launch_bounds__(256) head_pack_kernel(
   }
   __syncthreads();
   const unsigned mask = mask_s;
-  const int vecs = dim / 8;
-  for (int r = warp; r < PACK_ROWS; r += 8) {
+  const int vecs = p.dim / 8;
+  for (int r = warp; r < per; r += 8) {
     if (!((mask >> r) & 1u)) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(first + r) * ldx);
+    const uint4* src = reinterpret_cast<const uint4*>(p.x + (long long)(first + r) * p.ldx);
     uint4* dst = reinterpret_cast<uint4*>(
-        xp + (long long)(base_s + __popc(mask & ((1u << r) - 1))) * dim);
+        p.xp + (long long)(base_s + __popc(mask & ((1u << r) - 1))) * p.ldp);
+#pragma unroll 4
     for (int k = lane; k < vecs; k += 32) dst[k] = src[k];
   }
   if (blockIdx.x == gridDim.x - 1) {
     const int total = base_s + __popc(mask);
     const int stop = total > 64 ? (total + 63) / 64 * 64 : 64;
-    if (threadIdx.x == 0) *count = total;
-    for (int i = total + threadIdx.x; i < stop; i += 256) row_of[i] = -1;
-    uint4* z = reinterpret_cast<uint4*>(xp + (long long)total * dim);
-    for (long long k = threadIdx.x; k < (long long)(stop - total) * vecs; k += 256)
+    if (threadIdx.x == 0) *p.count = total;
+    // zero rows up to a whole block of 64, which dw's product reduces over
+    const int line = (int)(p.ldp / 8);
+    uint4* z = reinterpret_cast<uint4*>(p.xp + (long long)total * p.ldp);
+    for (long long k = threadIdx.x; k < (long long)(stop - total) * line; k += 256)
       z[k] = make_uint4(0, 0, 0, 0);
   }
 }
 
 // One warp per row: the softmax over the row's entries, then its ids sorted
 // with repeats added together (in the order of the entries), K^2 comparisons
-// out of shared memory.
+// out of shared memory, and an index: how many ids are below each multiple of
+// 256.
 constexpr int TEACHER_WARPS = 4;
 __global__ void __launch_bounds__(32 * TEACHER_WARPS) head_teacher_kernel(
     const int32_t* __restrict__ ids_in, const float* __restrict__ logit, int rows, int K, int vocab,
-    float inv_t, int* ids, float* prob, float* neg_entropy, int* keep, int* status) {
+    float inv_t, int* ids, float* prob, unsigned short* tab, int tab_ld, float* neg_entropy,
+    int* keep, int* status) {
   pdl_trigger();
   pdl_wait();
-  __shared__ int sid[TEACHER_WARPS][kTopkMax];
-  __shared__ float sp[TEACHER_WARPS][kTopkMax];
-  __shared__ int sfirst[TEACHER_WARPS][kTopkMax];
+  __shared__ __align__(16) int sid[TEACHER_WARPS][kTopkMax];
+  __shared__ __align__(16) float sp[TEACHER_WARPS][kTopkMax];
+  __shared__ __align__(16) int sfirst[TEACHER_WARPS][kTopkMax];
+  __shared__ int sorted[TEACHER_WARPS][kTopkMax];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.x * TEACHER_WARPS + w;
   if (r >= rows) return;
@@ -187,34 +226,62 @@ __global__ void __launch_bounds__(32 * TEACHER_WARPS) head_teacher_kernel(
   }
   ent = warp_sum(ent);
   __syncwarp();
+  // the entries up to a multiple of four are absent ones
+  const int K4 = (K + 3) & ~3;
+  if (lane < K4 - K) {
+    sid[w][K + lane] = INT_MAX;
+    sp[w][K + lane] = 0.f;
+    sfirst[w][K + lane] = INT_MAX;
+  }
   for (int k = lane; k < K; k += 32) {
     const int c = sid[w][k];
-    int first = c != INT_MAX;
-    for (int j = 0; j < k; ++j)
-      if (sid[w][j] == c) first = 0;
-    sfirst[w][k] = first;
+    int same = 0;   // an entry before it has the same id
+#pragma unroll 4
+    for (int j = 0; j < K4; j += 4) {
+      const int4 q = *reinterpret_cast<const int4*>(&sid[w][j]);
+      same |= (q.x == c && j < k) | (q.y == c && j + 1 < k) | (q.z == c && j + 2 < k) |
+              (q.w == c && j + 3 < k);
+    }
+    sfirst[w][k] = same ? INT_MAX : c;   // the id where it stands first
   }
   __syncwarp();
   int total = 0;
-  for (int k = lane; k < K; k += 32) total += sfirst[w][k];
+  for (int k = lane; k < K; k += 32) total += sfirst[w][k] != INT_MAX;
   total = __reduce_add_sync(0xffffffffu, total);
   for (int k = lane; k < K; k += 32) {
-    if (sfirst[w][k]) {
-      const int c = sid[w][k];
+    const int c = sfirst[w][k];
+    if (c != INT_MAX) {
       int rank = 0;
       float p = 0.f;
-      for (int j = 0; j < K; ++j) {
-        const int cj = sid[w][j];
-        rank += sfirst[w][j] && cj < c;
-        if (cj == c) p += sp[w][j];
+#pragma unroll 4
+      for (int j = 0; j < K4; j += 4) {
+        const int4 f = *reinterpret_cast<const int4*>(&sfirst[w][j]);
+        const int4 q = *reinterpret_cast<const int4*>(&sid[w][j]);
+        const float4 y4 = *reinterpret_cast<const float4*>(&sp[w][j]);
+        rank += (f.x < c) + (f.y < c) + (f.z < c) + (f.w < c);
+        p += q.x == c ? y4.x : 0.f;
+        p += q.y == c ? y4.y : 0.f;
+        p += q.z == c ? y4.z : 0.f;
+        p += q.w == c ? y4.w : 0.f;
       }
       ids[(long long)rank * rows + r] = c;
       prob[(long long)rank * rows + r] = p;
+      sorted[w][rank] = c;
     }
     if (k >= total) {
       ids[(long long)k * rows + r] = INT_MAX;
       prob[(long long)k * rows + r] = 0.f;
     }
+  }
+  __syncwarp();
+  for (int t = lane; t < tab_ld; t += 32) {
+    int lo = 0, hi = total;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sorted[w][mid] < t * HB_TAB) lo = mid + 1;
+      else hi = mid;
+    }
+    tab[(long long)r * tab_ld + t] = (unsigned short)lo;
   }
   if (lane == 0) {
     keep[r] = any;
@@ -306,7 +373,7 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
       for (int u = 0; u < SL; ++u) d += ssum[u][rl];
       loss = p.t2 * (p.neg_entropy[i] + kLn2 * d);
     } else if (on) {
-      loss = kLn2 * (lse2 - p.zt[i]);
+      loss = kLn2 * (lse2 - p.zt[m]);
     }
     p.loss[i] = loss;
     p.lse[i] = on ? kLn2 * lse2 : 0.f;
@@ -373,6 +440,7 @@ LsePlan lse_plan(int rows, int dim, int vocab, int num_sms) {
     const long long units = (long long)m_tiles * ((vocab + bn - 1) / bn);
     const double waves = (double)((units + p.clusters - 1) / p.clusters);
     const double cost = waves * (bn + 350 / dim_kb) + 6 * bn / dim_kb;
+    if (bn < 256 && p.packed && waves > 8) break;   // the rows that count are not known: 256
     if (bn == 256 || cost < best) {
       best = cost;
       p.bn = bn;
@@ -433,32 +501,56 @@ ne_status teacher_check(ne_ctx* ctx, const ne_teacher_desc* t, const char* what)
   return NE_OK;
 }
 
+int tab_entries(int vocab) { return (vocab + HB_TAB - 1) / HB_TAB; }
+
 ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
   if (!c.teacher) return NE_OK;
   HeadState* h = ctx->head;
   const int rows = c.d->rows;
   NE_LAUNCH(launch_k(head_teacher_kernel, dim3((rows + TEACHER_WARPS - 1) / TEACHER_WARPS),
                      dim3(32 * TEACHER_WARPS), 0, ctx->st, c.teacher->ids, c.teacher->logits, rows,
-                     c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->neg_entropy, h->keep,
-                     ctx->d_status));
+                     c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->tab, tab_entries(c.d->vocab),
+                     h->neg_entropy, h->keep, ctx->d_status));
   return NE_OK;
 }
 
-ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, int counters) {
+// lse: the backward pass's (NULL: forward)
+ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, const float* lse, const float* grad, int counters) {
   HeadState* h = ctx->head;
-  const int rows = c.d->rows;
-  NE_LAUNCH(launch_k(head_pack_kernel, dim3((rows + PACK_ROWS - 1) / PACK_ROWS), dim3(256), 0,
-                     ctx->st, (const __nv_bfloat16*)c.d->x, c.d->ldx, rows, c.d->dim, c.target,
-                     (const int*)(c.teacher ? h->keep : nullptr), c.d->vocab, h->row_of, h->pos_of,
-                     h->count, h->xp, h->counters, counters, ctx->d_status));
+  HeadPack p{};
+  p.x = (const __nv_bfloat16*)c.d->x;
+  p.ldx = c.d->ldx;
+  p.rows = c.d->rows;
+  p.dim = c.d->dim;
+  p.vocab = c.d->vocab;
+  p.per = pack_rows(p.rows);
+  p.target = c.target;
+  p.keep = c.teacher ? h->keep : nullptr;
+  p.row_of = h->row_of;
+  p.pos_of = h->pos_of;
+  p.count = h->count;
+  p.target_p = h->target;
+  p.xp = h->xp;
+  p.ldp = (long long)up(p.dim, GEMM_BK);
+  p.lse = lse;
+  p.grad = grad;
+  p.factor = c.t * c.d->scale;
+  p.coef = lse ? h->coef : nullptr;
+  p.counters = h->counters;
+  p.n_counters = counters;
+  p.status = ctx->d_status;
+  NE_LAUNCH(launch_k(head_pack_kernel, dim3((p.rows + p.per - 1) / p.per), dim3(256), 0, ctx->st, p));
   return NE_OK;
 }
 
+// Cross entropy's packed targets lie by packed row, a teacher's entries by row.
 HeadTargets targets_of(const HeadState* h, const HeadCall& c, bool packed) {
   HeadTargets t{};
-  t.ids = c.teacher ? h->ids : c.target;
+  t.ids = c.teacher ? h->ids : packed ? h->target : c.target;
   t.prob = c.teacher ? h->prob : nullptr;
-  t.row_of = packed ? h->row_of : nullptr;
+  t.row_of = packed && c.teacher ? h->row_of : nullptr;
+  t.tab = c.teacher ? h->tab : nullptr;
+  t.tab_ld = tab_entries(c.d->vocab);
   t.ld = c.d->rows;
   t.n = c.n;
   return t;
@@ -484,7 +576,7 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK) return s;
   const LsePlan plan = lse_plan(rows, D, V, ctx->num_sms);
-  if (plan.packed && (s = enqueue_pack(ctx, c, 0)) != NE_OK) return s;
+  if (plan.packed && (s = enqueue_pack(ctx, c, nullptr, nullptr, 0)) != NE_OK) return s;
   const int tile_m = GEMM_BM * plan.cg;
   const int n_tiles = (V + plan.bn - 1) / plan.bn;
   const long long units = (long long)((rows + tile_m - 1) / tile_m) * n_tiles;
@@ -508,7 +600,7 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   p.stages = plan.stages;
   p.one_row_tile = plan.one_row_tile;
   CUtensorMap x, w;
-  if (!make_tmap(&x, plan.packed ? h->xp : d.x, rows, D, plan.packed ? D : d.ldx, plan.a_rows, 0) ||
+  if (!make_tmap(&x, plan.packed ? h->xp : d.x, rows, D, plan.packed ? (long long)up(D, GEMM_BK) : d.ldx, plan.a_rows, 0) ||
       !make_tmap(&w, d.w, V, D, d.ldw, plan.bn / plan.cg, 0))
     return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
   if (plan.cg == 2) NE_LAUNCH(launch_lse<2>(x, w, p, plan, units, ctx->st));
@@ -558,12 +650,13 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
   p.piece = (int)up((vocab + p.pieces - 1) / p.pieces, HB_BN);
   p.pieces = (vocab + p.piece - 1) / p.piece;
   // dx's units are the longest: where there are few of them the piece is split
-  // until a unit is at most half of what a pair has to do in a step
+  // until a unit is a third of what a pair has to do for dx and dw (rows that do
+  // not count make that less than it looks from here), but not below 32
+  // k-blocks, twice what a unit's own hand-over and epilogue cost
   const double m_tiles = (double)((rows + p.tile_m - 1) / p.tile_m), d_tiles = (dim + HB_BN - 1) / HB_BN;
   const double piece_kb = p.piece / GEMM_BK;
-  double load = m_tiles * d_tiles * piece_kb + (p.piece / p.tile_m) * d_tiles * (double)(rows64 / GEMM_BK);
-  if (p.pieces > 1) load += m_tiles * (p.piece / HB_BN) * (double)((dim + GEMM_BK - 1) / GEMM_BK);
-  const double most = std::max(8.0, load / p.clusters / 2);
+  const double load = m_tiles * d_tiles * piece_kb + (p.piece / p.tile_m) * d_tiles * (double)(rows64 / GEMM_BK);
+  const double most = std::max(32.0, load / p.clusters / 3);
   const long long slabs = std::max<long long>(1, (long long)kSlabBytes / (rows64 * dim * 4));
   const long long want = std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
   p.split_n = (int)up((p.piece + want - 1) / want, GEMM_BK);
@@ -574,9 +667,8 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
 template <int CG>
 cudaError_t launch_step(const HeadMaps& maps, const HeadStep& step, const HeadDz& dz, int clusters,
                         cudaStream_t st) {
-  using C = GemmCfg<HB_BN, CG>;
   auto kern = head_step_kernel<CG>;
-  const size_t smem = C::SMEM_BYTES_STAGED;
+  const size_t smem = HeadCfg<CG>::SMEM;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   if constexpr (CG == 2)
@@ -594,20 +686,19 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   const HeadPlan plan = head_plan(rows, D, V, ctx->num_sms);
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK ||
-      (s = enqueue_pack(ctx, c, plan.pieces + 1)) != NE_OK)
+      (s = enqueue_pack(ctx, c, lse, grad, plan.pieces + 1)) != NE_OK)
     return s;
   HeadDz dz{};
   dz.t = targets_of(h, c, true);
-  dz.lse = lse;
-  dz.grad = grad;
+  dz.coef = h->coef;
   dz.c2 = d.scale / c.t * kLog2e;
-  dz.factor = c.t * d.scale;
+  const long long ldp = (long long)up(D, GEMM_BK);
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   HeadMaps maps;
-  bool ok = make_tmap(&maps.x_k, h->xp, rows64, D, D, GEMM_BM, 0) &&
+  bool ok = make_tmap(&maps.x_k, h->xp, rows64, D, ldp, GEMM_BM, 0) &&
             make_tmap(&maps.w_k, d.w, V, D, d.ldw, HB_BN / plan.cg, 0) &&
             make_tmap_mn(&maps.w_mn, d.w, D, V, d.ldw) &&
-            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, D) &&
+            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, ldp) &&
             make_tmap_out(&maps.dx_out, h->dx, plan.splits * rows64, D, D, f32, 4, 32);
   HeadStep step{};
   step.d_rows = h->count;
@@ -742,7 +833,8 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4),
                o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
                o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8),
-               o_xp = take(R256 * D * 2), o_dz0 = take(dz), o_dz1 = take(dz),
+               o_xp = take(R256 * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
+               o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz0 = take(dz), o_dz1 = take(dz),
                o_dx = take(std::max(up(R, 64) * D * 4, kSlabBytes)),
                o_counters = take((up(V, HB_BN) / HB_BN + 1) * 4);
   uint8_t* b = nullptr;
@@ -755,6 +847,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   n.keep = (int*)(b + o_keep);
   n.ids = (int*)(b + o_ids);
   n.prob = (float*)(b + o_prob);
+  n.target = (int*)(b + o_target);
+  n.coef = (float2*)(b + o_coef);
+  n.tab = (unsigned short*)(b + o_tab);
   n.neg_entropy = (float*)(b + o_ent);
   n.zt = (float*)(b + o_zt);
   n.stats = (float2*)(b + o_stats);
