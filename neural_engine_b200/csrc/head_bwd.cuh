@@ -1,19 +1,24 @@
-// head_bwd.cuh -- one step of the head losses' backward pass: the three
-// products of a piece of the vocabulary in one persistent launch.
+// head_bwd.cuh -- the head losses' backward pass: one persistent launch that
+// walks the vocabulary in pieces.
 //
-//   dz[p]  = f(x . w[p]^T)              rows x piece, K = dim
-//   dx    += dz[p-1] . w[p-1]           rows x dim,   K = piece (in splits)
-//   dw[p-1] = dz[p-1]^T . x             piece x dim,  K = rows
+//   dz[p] = f(x . w[p]^T)            rows x piece, K = dim
+//   dx   += dz[p] . w[p]             rows x dim,   K = piece (in splits)
+//   dw[p] = dz[p]^T . x              piece x dim,  K = rows
 //
-// Step p makes dz of piece p and uses that of piece p - 1, so the three have no
-// order among them and share the SMs: on their own they leave 14% of the pairs
-// idle in the last wave (4096 rows, dim 1024: 64 tiles of dx or 128 of dw for 74
-// pairs) and pay a launch each.  Work units are one 128 * CG x 256 tile (dx: of
-// one split of the piece); the leading CTA's producer draws them from a counter
-// in device memory, the longest kind first, and hands them to the other roles
-// of both CTAs through a ring of slots.  Which pair computes a unit changes no
-// value: every unit is computed whole, and what units of different steps add
-// into is ordered by the launches.
+// Bound by the tensor cores: 6 rows vocab dim operations, of which the first
+// product is the price of not keeping the logits.  Work units are one 128 * CG x
+// 256 tile (dx: of one split of the piece), in the order
+//   dz[0],  dz[1] dx[0] dw[0],  dz[2] dx[1] dw[1],  ...,  dx[P-1] dw[P-1]
+// so that what a unit reads was made a piece earlier, and pieces are small
+// enough to be read back from L2.  The leading CTA's A producer draws units from
+// a counter in device memory, waits until the units it depends on have
+// signalled, and hands it to the other roles of both CTAs through a ring of
+// slots.  A unit depends only on units drawn
+// before it, so the wait ends whatever the number of CTAs that run; it is
+// bounded all the same.  Which pair computes a unit changes no value: every
+// unit is computed whole, and dx adds the pieces in their order.
+// As launches of their own the products left 14% of the pairs idle in their last
+// waves (4096 rows, dim 1024: 64 tiles of dx, 128 of dw, for 74 pairs).
 //
 // Shared-memory ring, TMEM accumulators and CTA pairs are those of gemm_tc.cuh,
 // and so are the warp roles but for the producer: issuing a tensor load takes a
@@ -34,24 +39,32 @@ template <int CG>
 struct HeadCfg {
   static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + HB_BN / CG * GEMM_BK * 2;
-  static constexpr int STAGES = CG == 2 ? 5 : 3;
-  // ring, barriers, two boxes per epilogue warp, alignment
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 2048 + GEMM_EPI_WARPS * 2 * HB_BOX;
+  // a load takes up to 3,000 cycles to arrive and a k-block 512 to be used: as
+  // many stages as fit
+  static constexpr int STAGES = CG == 2 ? 6 : 4;
+  // ring, barriers, a box per epilogue warp, alignment
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 2048 + GEMM_EPI_WARPS * HB_BOX;
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
-struct HeadStep {
+constexpr int HB_BUFS = 3;   // pieces of dz alive: made, waited for, read
+
+struct HeadWalk {
   const int* d_rows;        // packed rows
-  int* counter;             // next work unit, zero at launch
+  int* counters;            // units drawn, then three per piece, all zero at launch
   int* status;
-  int rows64;               // slab height of dx
-  int dim, dim_kb, dim_tiles;   // dim, in k-blocks of 64 and in tiles of 256
-  // piece p (dz): first id, ids (0: none)
-  int make0, make_n;
-  // piece p - 1 (dx, dw): first id, ids (0: none), ids per dx split (a multiple of 64)
-  int use0, use_n, split_n, splits;
-  int want_dx, want_dw, dx_add, dw_f32;
+  int rows64;               // rows of a dz buffer and of a slab of dx
+  int vocab, dim, dim_kb, dim_tiles;   // dim also in k-blocks of 64 and tiles of 256
+  int piece, pieces;        // ids a piece (a multiple of 256)
+  int split_n;              // ids a split of dx's product (a multiple of 64)
+  int want_dx, want_dw, dw_f32;
 };
+// counters of piece p: dz written (per epilogue warp), dz read (per unit), dx
+// added (per epilogue warp)
+enum HeadFlag : int { HF_MADE = 0, HF_READ = 1, HF_ADDED = 2 };
+__device__ __forceinline__ int* head_flag(const HeadWalk& s, int p, int what) {
+  return s.counters + 1 + 3 * p + what;
+}
 
 // The sparse targets of the rows: sorted ids, [entry][row], INT_MAX behind the
 // last.
@@ -100,81 +113,168 @@ struct HeadDz {
 
 struct HeadMaps {
   CUtensorMap x_k, w_k;        // dz: operands (K = dim contiguous)
-  CUtensorMap dz_out;          // dz: piece p
-  CUtensorMap dz_k, w_mn;      // dx: dz of piece p - 1 (K = ids), w as [ids][dim]
+  CUtensorMap dz_out;          // dz: [buffers * rows64][piece]
+  CUtensorMap dz_k, w_mn;      // dx: dz (K = ids), w as [ids][dim]
   CUtensorMap dx_out;          // dx: [splits * rows64][dim] fp32
   CUtensorMap dz_mn, x_mn;     // dw: both as [rows][...]
-  CUtensorMap dw_out;
+  CUtensorMap dw_out;          // dw: [vocab][dim]
 };
 
-enum HeadKind : int { HK_DX = 0, HK_DW = 1, HK_DZ = 2 };
+enum HeadKind : int { HK_DX = 0, HK_DW = 1, HK_DZ = 2, HK_END = 3 };
 
 struct HeadUnit {
-  int kind, mt, nt, split, kb0, kb;
+  int kind, piece, mt, nt, split, kb0, kb;
   int n;   // columns: 256, or what is left of them in whole 32s
 };
+
+// Units of each kind in a piece of `ids` ids.
+struct HeadCounts {
+  int dz, dx, dw;
+};
+__device__ __forceinline__ HeadCounts head_counts(const HeadWalk& s, int m_tiles, int tile_m, int ids) {
+  HeadCounts c;
+  c.dz = m_tiles * ((ids + HB_BN - 1) / HB_BN);
+  c.dx = s.want_dx ? m_tiles * s.dim_tiles * ((ids + s.split_n - 1) / s.split_n) : 0;
+  c.dw = s.want_dw ? s.dim_tiles * ((ids + tile_m - 1) / tile_m) : 0;
+  return c;
+}
 
 __device__ __forceinline__ int unit_cols(int cols, int nt) {
   return min(HB_BN, (cols - nt * HB_BN + 31) & ~31);
 }
 
-// unit u of the step, dx first (the longest), dz last
-__device__ __forceinline__ bool head_unit(const HeadStep& s, int rows_blocks, int m_tiles, int tile_m,
-                                          int u, HeadUnit& o) {
-  const int n_dx = s.use_n && s.want_dx ? m_tiles * s.dim_tiles * s.splits : 0;
-  o.split = 0;
-  o.kb0 = 0;
-  if (u < n_dx) {
-    o.kind = HK_DX;
-    o.nt = u % s.dim_tiles;
+// Where the walk stands: what every role derives once from the number of rows.
+struct HeadOrder {
+  int blocks, m_tiles, tile_m;
+  int last_ids;              // of the last piece
+  HeadCounts full, last;     // units of a whole piece and of the last one
+};
+
+// unit u of the walk (HK_END behind the last one)
+__device__ __forceinline__ void head_unit(const HeadWalk& s, const HeadOrder& o, int u, HeadUnit& w) {
+  const int P = s.pieces;
+  const int made0 = P > 1 ? o.full.dz : o.last.dz;
+  int kind_at = -1;   // position among dz, dx, dw units of one phase
+  int made = -1, used = -1;
+  if (u < made0) {
+    made = 0;
+    kind_at = u;
+  } else {
+    u -= made0;
+    // phase q makes piece q + 1 and uses piece q; the last one makes none
+    const int phase = o.full.dz + o.full.dx + o.full.dw;
+    const int whole = max(P - 2, 0);
+    int q = min(u / phase, whole);
+    u -= q * phase;
+    if (q == whole && P > 1) {
+      const int n = o.last.dz + o.full.dx + o.full.dw;
+      if (u >= n) {
+        u -= n;
+        ++q;
+      }
+    }
+    used = q;
+    const int dz_n = q + 1 >= P ? 0 : q + 1 == P - 1 ? o.last.dz : o.full.dz;
+    if (u < dz_n) {
+      made = q + 1;
+      kind_at = u;
+    } else {
+      u -= dz_n;
+    }
+  }
+  w.split = 0;
+  w.mt = w.nt = 0;
+  w.kb0 = w.kb = 0;
+  if (made >= 0) {
+    w.kind = HK_DZ;
+    w.piece = made;
+    w.mt = kind_at % o.m_tiles;
+    w.nt = kind_at / o.m_tiles;
+    w.kb = s.dim_kb;
+    w.n = unit_cols(made == P - 1 ? o.last_ids : s.piece, w.nt);
+    return;
+  }
+  const HeadCounts& c = used == P - 1 ? o.last : o.full;
+  const int ids = used == P - 1 ? o.last_ids : s.piece;
+  w.piece = used;
+  if (u < c.dx) {
+    w.kind = HK_DX;
+    w.nt = u % s.dim_tiles;
     const int r = u / s.dim_tiles;
-    o.mt = r % m_tiles;
-    o.split = r / m_tiles;
-    o.kb0 = o.split * (s.split_n / GEMM_BK);
-    const int left = s.use_n - o.split * s.split_n;
-    o.kb = (min(left, s.split_n) + GEMM_BK - 1) / GEMM_BK;
-    o.n = unit_cols(s.dim, o.nt);
-    return true;
+    w.mt = r % o.m_tiles;
+    w.split = r / o.m_tiles;
+    w.kb0 = w.split * (s.split_n / GEMM_BK);
+    w.kb = (min(ids - w.split * s.split_n, s.split_n) + GEMM_BK - 1) / GEMM_BK;
+  } else if (u - c.dx < c.dw) {
+    u -= c.dx;
+    w.kind = HK_DW;
+    w.nt = u % s.dim_tiles;
+    w.mt = u / s.dim_tiles;
+    w.kb = o.blocks;
+  } else {
+    w.kind = HK_END;
   }
-  u -= n_dx;
-  const int v_tiles = (s.use_n + tile_m - 1) / tile_m;
-  const int n_dw = s.want_dw ? v_tiles * s.dim_tiles : 0;
-  if (u < n_dw) {
-    o.kind = HK_DW;
-    o.nt = u % s.dim_tiles;
-    o.mt = u / s.dim_tiles;
-    o.kb = rows_blocks;
-    o.n = unit_cols(s.dim, o.nt);
-    return true;
-  }
-  u -= n_dw;
-  if (u < m_tiles * ((s.make_n + HB_BN - 1) / HB_BN)) {
-    o.kind = HK_DZ;
-    o.mt = u % m_tiles;
-    o.nt = u / m_tiles;
-    o.kb = s.dim_kb;
-    o.n = unit_cols(s.make_n, o.nt);
-    return true;
-  }
-  return false;
+  w.n = unit_cols(s.dim, w.nt);
 }
 
-// Arrivals and writes across the pair.  The data that crosses is one int a work
-// unit, written together with its completion (st.async), so nothing has to be
+__device__ __forceinline__ void flag_add(int* f) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(f) : "memory");
+}
+__device__ __forceinline__ bool flag_reached(const int* f, int want) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
+  return v >= want;
+}
+// Bounded wait until *f >= want.
+__device__ __forceinline__ bool flag_wait(const int* f, int want, int* status, volatile int* abort) {
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (flag_reached(f, want)) return true;
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > kWaitBudgetNs) {
+      atomicExch(status, DEV_ERR_TIMEOUT);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+// What was written through TMA before a flag is read through TMA after it.
+__device__ __forceinline__ void fence_async_global() {
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+// Arrivals and writes across the pair.  The data that crosses is a work unit,
+// written together with its completion (st.async), so nothing has to be
 // fenced at cluster scope: such a release costs an epilogue warp about 1,400
 // cycles, and the matching acquire another 1,000.
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ void post_int(uint32_t cluster_addr, uint32_t cluster_bar, int v) {
-  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], 4;" ::"r"(
+__device__ __forceinline__ void post_unit(uint32_t cluster_addr, uint32_t cluster_bar,
+                                          const HeadUnit& w) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], 32;" ::"r"(
                    cluster_bar)
                : "memory");
   asm volatile(
-      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(
-          cluster_addr),
-      "r"(v), "r"(cluster_bar)
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, "
+      "[%5];" ::"r"(cluster_addr),
+      "r"(w.kind), "r"(w.piece), "r"(w.mt), "r"(w.nt), "r"(cluster_bar)
       : "memory");
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, "
+      "[%5];" ::"r"(cluster_addr + 16),
+      "r"(w.split), "r"(w.kb0), "r"(w.kb), "r"(w.n), "r"(cluster_bar)
+      : "memory");
+}
+__device__ __forceinline__ void read_unit(uint32_t addr, HeadUnit& w) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w.kind), "=r"(w.piece), "=r"(w.mt), "=r"(w.nt)
+               : "r"(addr)
+               : "memory");
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w.split), "=r"(w.kb0), "=r"(w.kb), "=r"(w.n)
+               : "r"(addr + 16)
+               : "memory");
 }
 
 // 32 values to bf16, the low 16 bits of each word first.
@@ -221,14 +321,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 
 template <int CG>
 __global__ void __launch_bounds__(HB_THREADS, 1)
-head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const HeadDz dzp) {
+head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const HeadDz dzp) {
   using C = HeadCfg<CG>;
   constexpr bool PAIR = CG == 2;
   constexpr int TILE_M = GEMM_BM * CG;
   constexpr int STAGES = C::STAGES;
   constexpr uint32_t TMEM_COLS = 2 * HB_BN;
   constexpr uint32_t MN_BOX = 64 * GEMM_BK * 2;
-  constexpr int B_ROWS = HB_BN / CG;
   // readers of a slot: the MMA thread, B's producer and 8 epilogue warps, and the
   // other CTA's producers and epilogue warps
   constexpr int SLOT_READERS = CG * (2 + GEMM_EPI_WARPS);
@@ -246,8 +345,8 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
   const uint32_t drain_bar = tempty_bar + 16;             // [1]
   const uint32_t sfull_bar = drain_bar + 8;               // [HB_SLOTS]
   const uint32_t sempty_bar = sfull_bar + 8 * HB_SLOTS;   // [HB_SLOTS], the leader's
-  const uint32_t slots = sempty_bar + 8 * HB_SLOTS;       // [HB_SLOTS] int
-  const uint32_t misc = slots + 4 * HB_SLOTS;
+  const uint32_t misc = sempty_bar + 8 * HB_SLOTS;
+  const uint32_t slots = bars + 512;                      // [HB_SLOTS] units of 32 bytes
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + (misc - base));
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + (misc - base) + 4);
 
@@ -288,17 +387,24 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
+  // the leader's A producer draws its first unit while the row count arrives
+  int drawn = threadIdx.x == 0 && crank == 0 ? atomicAdd(sp.counters, 1) : 0;
   // whole blocks of 64 rows, at least one (its rows are zeros)
   const int count = *sp.d_rows;
-  const int blocks = max((count + GEMM_BK - 1) / GEMM_BK, 1);
-  const int M = blocks * GEMM_BK;
-  const int m_tiles = (M + TILE_M - 1) / TILE_M;
+  HeadOrder ord;
+  ord.blocks = max((count + GEMM_BK - 1) / GEMM_BK, 1);
+  ord.tile_m = TILE_M;
+  const int M = ord.blocks * GEMM_BK;
+  ord.m_tiles = (M + TILE_M - 1) / TILE_M;
+  ord.last_ids = sp.vocab - (sp.pieces - 1) * sp.piece;
+  ord.full = head_counts(sp, ord.m_tiles, TILE_M, sp.piece);
+  ord.last = head_counts(sp, ord.m_tiles, TILE_M, ord.last_ids);
 
   // a role other than the leader's producer takes the unit of slot `it`
-  auto take = [&](int it, int& u) -> bool {
+  auto take = [&](int it, HeadUnit& w) -> bool {
     const int s = it % HB_SLOTS;
     if (!mbar_wait(sfull_bar + 8 * s, (it / HB_SLOTS) & 1, sp.status, abort_flag)) return false;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(slots + 4 * s) : "memory");
+    read_unit(slots + 32 * s, w);
     return true;
   };
   auto taken = [&](int it) {
@@ -322,32 +428,75 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      int drawn = leads ? atomicAdd(sp.counter, 1) : 0;
+      HeadUnit nw{};   // the leader's next unit
+      // hands over the leader's next unit once what it depends on is done: dz,
+      // its buffer was read for the last time; dx and dw, dz was written, and dx
+      // was added to by the piece before.  now: wait for that.
+      auto hand_over = [&](int it, bool now) -> bool {
+        const int* f[2] = {nullptr, nullptr};
+        int want[2] = {0, 0};
+        if (nw.kind == HK_DZ) {
+          if (nw.piece >= HB_BUFS) {
+            f[0] = head_flag(sp, nw.piece - HB_BUFS, HF_READ);
+            want[0] = ord.full.dx + ord.full.dw;
+          }
+        } else if (nw.kind != HK_END) {
+          f[0] = head_flag(sp, nw.piece, HF_MADE);
+          want[0] = (nw.piece == sp.pieces - 1 ? ord.last.dz : ord.full.dz) * CG * GEMM_EPI_WARPS;
+          if (nw.kind == HK_DX && nw.piece > 0) {
+            f[1] = head_flag(sp, nw.piece - 1, HF_ADDED);
+            want[1] = ord.full.dx * CG * GEMM_EPI_WARPS;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!f[i] || flag_reached(f[i], want[i])) continue;
+          if (!now) return false;
+          if (!flag_wait(f[i], want[i], sp.status, abort_flag)) {
+            ok = false;
+            return false;
+          }
+        }
+        const int s = it % HB_SLOTS;
+        const uint32_t at = slots + 32 * s;
+        if (!mbar_wait(sempty_bar + 8 * s, ((it / HB_SLOTS) & 1) ^ 1, sp.status, abort_flag)) {
+          ok = false;
+          return false;
+        }
+        st_shared_v4(at, nw.kind, nw.piece, nw.mt, nw.nt);
+        st_shared_v4(at + 16, nw.split, nw.kb0, nw.kb, nw.n);
+        mbar_arrive(sfull_bar + 8 * s);
+        if constexpr (PAIR) post_unit(mapa_shared(at, 1), mapa_shared(sfull_bar + 8 * s, 1), nw);
+        return true;
+      };
+      if (leads) {
+        head_unit(sp, ord, drawn, nw);
+        hand_over(0, true);
+      }
       for (int it = 0; ok; ++it) {
-        int u;
+        HeadUnit w;
+        bool handed = false;
         if (leads) {
-          u = drawn;
-          const int s = it % HB_SLOTS;
-          if (!mbar_wait(sempty_bar + 8 * s, ((it / HB_SLOTS) & 1) ^ 1, sp.status, abort_flag)) break;
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(slots + 4 * s), "r"(u) : "memory");
-          mbar_arrive(sfull_bar + 8 * s);
-          if constexpr (PAIR) post_int(mapa_shared(slots + 4 * s, 1), mapa_shared(sfull_bar + 8 * s, 1), u);
+          w = nw;
+          if (w.kind != HK_END) drawn = atomicAdd(sp.counters, 1);   // arrives behind the loads
         } else {
-          if (!take(it, u)) break;
+          if (!take(it, w)) break;
           taken(it);
         }
-        HeadUnit w;
-        if (!head_unit(sp, blocks, m_tiles, TILE_M, u, w)) break;
-        if (leads) drawn = atomicAdd(sp.counter, 1);   // its latency passes behind the loads
+        if (w.kind == HK_END) break;
+        fence_async_global();
+        const int buf_row = (w.piece % HB_BUFS) * sp.rows64, id0 = w.piece * sp.piece;
         // this role's operand: K-major is one box, MN-major one per 64 columns
         const bool mn = is_a ? w.kind == HK_DW : w.kind != HK_DZ;
         const CUtensorMap* tm =
             is_a ? (w.kind == HK_DZ ? &maps.x_k : w.kind == HK_DX ? &maps.dz_k : &maps.dz_mn)
                  : (w.kind == HK_DZ ? &maps.w_k : w.kind == HK_DX ? &maps.w_mn : &maps.x_mn);
         // first row (K-major) or column (MN-major) of the tile, and where K starts
-        const int first = is_a ? w.mt * TILE_M + (int)crank * GEMM_BM
-                               : w.nt * HB_BN + (int)crank * (w.n / CG) + (w.kind == HK_DZ ? sp.make0 : 0);
-        int k0 = w.kb0 * GEMM_BK + (!is_a && w.kind == HK_DX ? sp.use0 : 0);
+        const int first = is_a ? w.mt * TILE_M + (int)crank * GEMM_BM + (w.kind == HK_DX ? buf_row : 0)
+                               : w.nt * HB_BN + (int)crank * (w.n / CG) + (w.kind == HK_DZ ? id0 : 0);
+        int k0 = w.kb0 * GEMM_BK;
+        if (is_a && w.kind == HK_DW) k0 += buf_row;
+        if (!is_a && w.kind == HK_DX) k0 += id0;
         for (int k = 0; k < w.kb; ++k, k0 += GEMM_BK) {
           const uint32_t bar = full_to + 8 * stage;
           const uint32_t dst = tiles + stage * C::STAGE_BYTES + (is_a ? 0 : C::A_BYTES);
@@ -367,6 +516,15 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
             }
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (leads && k == 1) {   // the loads are ahead of the MMAs now: time for the next unit
+            head_unit(sp, ord, drawn, nw);
+            handed = hand_over(it + 1, false);
+            if (!ok) break;
+          }
+        }
+        if (leads && ok && !handed) {
+          if (w.kb < 2) head_unit(sp, ord, drawn, nw);
+          hand_over(it + 1, true);
         }
       }
       // no load may be in flight when the CTA exits (gemm_tc.cuh)
@@ -388,11 +546,10 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
       int acc = 0;
       uint32_t acc_phase = 0;
       for (int it = 0;; ++it) {
-        int u;
-        if (!take(it, u)) break;
-        taken(it);
         HeadUnit w;
-        if (!head_unit(sp, blocks, m_tiles, TILE_M, u, w)) break;
+        if (!take(it, w)) break;
+        taken(it);
+        if (w.kind == HK_END) break;
         if (!mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, sp.status, abort_flag)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * HB_BN;
@@ -434,17 +591,32 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
     // ------------------------------------------------ epilogue (warps 2..9)
     const int quarter = warp & 3;
     const int half = (warp - 2) >> 2;
-    const uint32_t sbuf = base + STAGES * C::STAGE_BYTES + 1024 + (warp - 2) * 2 * HB_BOX;
+    const uint32_t sbuf = base + STAGES * C::STAGE_BYTES + 1024 + (warp - 2) * HB_BOX;
     int acc = 0;
     uint32_t acc_phase = 0;
+    // The unit whose stores others wait for: signalled when they are complete,
+    // which costs nothing once the next unit's boxes or accumulator are due.
+    // Never kept over a wait.
+    int* owed = nullptr;
+    auto settle = [&] {   // lane 0
+      bulk_wait_all();
+      if (owed) {
+        fence_async_global();
+        flag_add(owed);
+        owed = nullptr;
+      }
+    };
     for (int it = 0;; ++it) {
-      int u = 0;
-      const bool got = take(it, u);
+      if (lane == 0 && owed && !mbar_try_wait(sfull_bar + 8 * (it % HB_SLOTS), (it / HB_SLOTS) & 1))
+        settle();
+      HeadUnit w;
+      const bool got = take(it, w);
       if (!__all_sync(0xffffffffu, got)) break;
       __syncwarp();
       if (lane == 0) taken(it);
-      HeadUnit w;
-      if (!head_unit(sp, blocks, m_tiles, TILE_M, u, w)) break;
+      if (w.kind == HK_END) break;
+      const int id0 = w.piece * sp.piece;
+      const int ids = w.piece == sp.pieces - 1 ? ord.last_ids : sp.piece;
       const int y0 = w.mt * TILE_M + (int)crank * GEMM_BM + quarter * 32;   // the warp's first row
       const int n_tile = w.nt * HB_BN;
       // |dz| = 2^(c2 acc - lse2 + log2|a|) - |a| p: the coefficient goes into the
@@ -461,80 +633,84 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
           keep = 0xffffffffu;
           sign = co.x < 0.f ? 0x80008000u : 0u;
         }
-        cursor_seek(dzp.t, cur, m, count, sp.make0 + n_tile + 128 * half);
+        cursor_seek(dzp.t, cur, m, count, id0 + n_tile + 128 * half);
       }
+      if (lane == 0 && owed && !mbar_try_wait(tfull_bar + 8 * acc, acc_phase)) settle();
       const bool ready = mbar_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag);
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * HB_BN;
       const bool b16 = w.kind == HK_DZ || (w.kind == HK_DW && !sp.dw_f32);
-      const bool rows_in = y0 < (w.kind == HK_DW ? sp.use_n : M);
-      const int cols_end = w.kind == HK_DZ ? sp.make_n : sp.dim;
+      const bool rows_in = y0 < (w.kind == HK_DW ? ids : M);
+      // dz in whole k-blocks of 64 ids: dx's product reads them
+      const int cols_end = w.kind == HK_DZ ? (ids + 63) & ~63 : sp.dim;
+      // dz has been read, as far as this unit is concerned
+      if (w.kind != HK_DZ && warp == 2 && lane == 0 && crank == 0)
+        flag_add(head_flag(sp, w.piece, HF_READ));
       const CUtensorMap* out = w.kind == HK_DZ ? &maps.dz_out
                                : w.kind == HK_DW ? &maps.dw_out : &maps.dx_out;
-      // a warp owns half of the tile's columns and sends boxes of 128-byte rows,
-      // 64 columns of bf16 or 32 of fp32, two at a time: the fence between the
-      // writes of a box and its store costs about 600 cycles
+      // a warp owns half of the tile's columns and sends boxes of 128-byte rows:
+      // 64 columns of bf16 or 32 of fp32 at a time
       const int step = b16 ? 64 : 32;
-      const bool add = w.kind == HK_DX ? sp.dx_add : w.kind == HK_DW && sp.dw_f32;
-      const int y = w.kind == HK_DX ? w.split * sp.rows64 + y0 : y0;
+      const bool add = w.kind == HK_DX ? w.piece > 0 : w.kind == HK_DW && sp.dw_f32;
+      const int y = y0 + (w.kind == HK_DX ? w.split * sp.rows64
+                          : w.kind == HK_DW ? id0 : (w.piece % HB_BUFS) * sp.rows64);
 #pragma unroll 1
-      for (int c0 = 128 * half; c0 < 128 * half + 128; c0 += 2 * step) {
-        if (n_tile + c0 >= cols_end) break;
-        if (lane == 0) bulk_wait_read_all();   // the previous boxes have left
-        __syncwarp();
-#pragma unroll 1
-        for (int b = 0; b < 2; ++b) {
-          const int c = c0 + b * step, n0 = n_tile + c;
-          if (n0 >= cols_end) break;
-          uint32_t o[32];
-          if (b16) {
+      for (int c = 128 * half; c < 128 * half + 128; c += step) {
+        const int n0 = n_tile + c;
+        if (n0 >= cols_end) break;
+        uint32_t o[32];
+        if (b16) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float v[32];
-              tmem_ld32(t_row + c + 32 * h, v);
-              if (w.kind == HK_DZ) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
-                const int col = sp.make0 + n0 + 32 * h;
-                while (cur.next < col + 32) {
-                  if (cur.next >= col) {
-                    const int j = cur.next - col;
-                    const float q = dzp.t.prob ? dzp.t.prob[cur.at * dzp.t.ld + cur.row] : 1.0f;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                      if (i == j) v[i] -= mag * q;
-                  }
-                  cursor_step(dzp.t, cur);
-                }
-              }
-              // rounded once to bf16: dz is the operand of two tensor-core
-              // products, dw the caller's type
-              pack_bf16(v, o + 16 * h);
-            }
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            tmem_ld32(t_row + c + 32 * h, v);
             if (w.kind == HK_DZ) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
-            }
-          } else {
-            float v[32];
-            tmem_ld32(t_row + c, v);
+              for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
+              if (n0 + 32 * h + 32 > ids) {   // behind the last id of the vocabulary
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
+                for (int j = 0; j < 32; ++j)
+                  if (n0 + 32 * h + j >= ids) v[j] = 0.f;
+              }
+              const int col = id0 + n0 + 32 * h;
+              while (cur.next < col + 32) {
+                if (cur.next >= col) {
+                  const int j = cur.next - col;
+                  const float q = dzp.t.prob ? dzp.t.prob[cur.at * dzp.t.ld + cur.row] : 1.0f;
+#pragma unroll
+                  for (int i = 0; i < 32; ++i)
+                    if (i == j) v[i] -= mag * q;
+                }
+                cursor_step(dzp.t, cur);
+              }
+            }
+            // rounded once to bf16: dz is the operand of two tensor-core
+            // products, dw the caller's type
+            pack_bf16(v, o + 16 * h);
           }
-          stage_words(sbuf + b * HB_BOX, lane, o);
+          if (w.kind == HK_DZ) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
+          }
+        } else {
+          float v[32];
+          tmem_ld32(t_row + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
         }
+        if (lane == 0) {   // the previous box has left the slot
+          if (owed) settle();
+          else bulk_wait_read_all();
+        }
+        __syncwarp();
+        stage_words(sbuf, lane, o);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
           if (rows_in) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const int n0 = n_tile + c0 + b * step;
-              if (n0 >= cols_end) break;
-              if (add) tma_reduce_add_2d(out, sbuf + b * HB_BOX, n0, y);
-              else tma_store_2d(out, sbuf + b * HB_BOX, n0, y);
-            }
+            if (add) tma_reduce_add_2d(out, sbuf, n0, y);
+            else tma_store_2d(out, sbuf, n0, y);
           }
           bulk_commit_group();
         }
@@ -544,10 +720,15 @@ head_step_kernel(const __grid_constant__ HeadMaps maps, const HeadStep sp, const
       if (lane == 0) {
         if constexpr (PAIR) mbar_arrive_peer(mapa_shared(tempty_bar + 8 * acc, 0));
         else mbar_arrive(tempty_bar + 8 * acc);
+        // others wait for what this unit wrote
+        if (w.kind != HK_DW) {
+          if (owed) settle();   // a unit without a box of its own
+          owed = head_flag(sp, w.piece, w.kind == HK_DZ ? HF_MADE : HF_ADDED);
+        }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
-    if (lane == 0) bulk_wait_all();
+    if (lane == 0) settle();
   }
 
   tc_fence_before();

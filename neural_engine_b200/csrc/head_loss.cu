@@ -57,9 +57,9 @@ struct HeadState {
   float* zt = nullptr;            // [topk][rows] target logits, log2 units
   float2* stats = nullptr;        // (max, sum exp2) of each row and half tile
   __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim up to 64] packed x
-  __nv_bfloat16* dz[2] = {};      // the pieces of dz that are made and used
+  __nv_bfloat16* dz = nullptr;    // [3][rows up to 64][piece]
   float* dx = nullptr;            // [splits][rows up to 64][dim] sums over the pieces
-  int* counters = nullptr;        // work units drawn, one per backward step
+  int* counters = nullptr;        // of the backward pass: units drawn, three per piece
 };
 
 namespace {
@@ -68,8 +68,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kTopkMax = 256;
-// dz of one piece (two are alive), and the slabs dx is summed in where its
-// product is split
+// dz of one piece (three are alive), and the slabs dx is summed in where its
+// product is split.  4096 rows of 151936 ids, dim 1024, backward pass: 3.41 ms with
+// pieces of 32 MB, 3.26 with 64, 3.18 with 128, 3.11 with 256 (1.2 GB would be
+// all of dz): longer sums per unit of dx against room.
 constexpr size_t kPieceBytes = 128u << 20;
 constexpr size_t kSlabBytes = 64u << 20;
 
@@ -665,16 +667,16 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
 }
 
 template <int CG>
-cudaError_t launch_step(const HeadMaps& maps, const HeadStep& step, const HeadDz& dz, int clusters,
+cudaError_t launch_walk(const HeadMaps& maps, const HeadWalk& walk, const HeadDz& dz, int clusters,
                         cudaStream_t st) {
-  auto kern = head_step_kernel<CG>;
+  auto kern = head_walk_kernel<CG>;
   const size_t smem = HeadCfg<CG>::SMEM;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   if constexpr (CG == 2)
-    return launch_k_cluster(kern, dim3(2 * clusters), dim3(HB_THREADS), smem, st, 2u, maps, step, dz);
+    return launch_k_cluster(kern, dim3(2 * clusters), dim3(HB_THREADS), smem, st, 2u, maps, walk, dz);
   else
-    return launch_k(kern, dim3(clusters), dim3(HB_THREADS), smem, st, maps, step, dz);
+    return launch_k(kern, dim3(clusters), dim3(HB_THREADS), smem, st, maps, walk, dz);
 }
 
 ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const float* grad,
@@ -686,59 +688,45 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   const HeadPlan plan = head_plan(rows, D, V, ctx->num_sms);
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK ||
-      (s = enqueue_pack(ctx, c, lse, grad, plan.pieces + 1)) != NE_OK)
+      (s = enqueue_pack(ctx, c, lse, grad, 1 + 3 * plan.pieces)) != NE_OK)
     return s;
   HeadDz dz{};
   dz.t = targets_of(h, c, true);
   dz.coef = h->coef;
   dz.c2 = d.scale / c.t * kLog2e;
-  const long long ldp = (long long)up(D, GEMM_BK);
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const long long ldp = (long long)up(D, GEMM_BK);
+  const int esz = g->dw_f32 ? 4 : 2, dz_rows = HB_BUFS * rows64;
   HeadMaps maps;
   bool ok = make_tmap(&maps.x_k, h->xp, rows64, D, ldp, GEMM_BM, 0) &&
             make_tmap(&maps.w_k, d.w, V, D, d.ldw, HB_BN / plan.cg, 0) &&
+            make_tmap_out(&maps.dz_out, h->dz, dz_rows, plan.piece, plan.piece, bf, 2, 64) &&
+            make_tmap(&maps.dz_k, h->dz, dz_rows, plan.piece, plan.piece, GEMM_BM, 0) &&
             make_tmap_mn(&maps.w_mn, d.w, D, V, d.ldw) &&
-            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, ldp) &&
-            make_tmap_out(&maps.dx_out, h->dx, plan.splits * rows64, D, D, f32, 4, 32);
-  HeadStep step{};
-  step.d_rows = h->count;
-  step.status = ctx->d_status;
-  step.rows64 = rows64;
-  step.dim = D;
-  step.dim_kb = (D + GEMM_BK - 1) / GEMM_BK;
-  step.dim_tiles = (D + HB_BN - 1) / HB_BN;
-  step.split_n = plan.split_n;
-  step.want_dx = g->dx != nullptr;
-  step.want_dw = g->dw != nullptr;
-  step.dw_f32 = g->dw_f32 != 0;
-  const int esz = g->dw_f32 ? 4 : 2;
-  const int ldz = plan.piece;
-  for (int p = 0; ok && p <= plan.pieces; ++p) {
-    step.counter = h->counters + p;
-    step.make0 = p * plan.piece;
-    step.make_n = p < plan.pieces ? std::min(plan.piece, V - step.make0) : 0;
-    step.use0 = (p - 1) * plan.piece;
-    step.use_n = p > 0 ? std::min(plan.piece, V - step.use0) : 0;
-    step.splits = (step.use_n + plan.split_n - 1) / plan.split_n;
-    step.dx_add = p > 1;
-    // a kind without units keeps another step's maps, which nothing reads
-    if (step.make_n)
-      ok = make_tmap_out(&maps.dz_out, h->dz[p & 1], rows64, step.make_n, ldz, bf, 2, 64);
-    if (ok && p > 0) {
-      const __nv_bfloat16* z = h->dz[(p - 1) & 1];
-      ok = make_tmap(&maps.dz_k, z, rows64, step.use_n, ldz, GEMM_BM, 0) &&
-           make_tmap_mn(&maps.dz_mn, z, step.use_n, rows64, ldz);
-      if (ok && g->dw)
-        ok = make_tmap_out(&maps.dw_out, (uint8_t*)g->dw + (long long)step.use0 * g->lddw * esz,
-                           step.use_n, D, g->lddw, g->dw_f32 ? f32 : bf, esz, 128 / esz);
-    } else if (ok) {
-      maps.dz_k = maps.dz_mn = maps.dw_out = maps.dz_out;
-    }
-    if (!ok) break;
-    if (plan.cg == 2) NE_LAUNCH(launch_step<2>(maps, step, dz, plan.clusters, ctx->st));
-    else NE_LAUNCH(launch_step<1>(maps, step, dz, plan.clusters, ctx->st));
-  }
+            make_tmap_out(&maps.dx_out, h->dx, plan.splits * rows64, D, D, f32, 4, 32) &&
+            make_tmap_mn(&maps.dz_mn, h->dz, plan.piece, dz_rows, plan.piece) &&
+            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, ldp);
+  maps.dw_out = maps.dx_out;   // not used without dw
+  if (ok && g->dw)
+    ok = make_tmap_out(&maps.dw_out, g->dw, V, D, g->lddw, g->dw_f32 ? f32 : bf, esz, 128 / esz);
   if (!ok) return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
+  HeadWalk walk{};
+  walk.d_rows = h->count;
+  walk.counters = h->counters;
+  walk.status = ctx->d_status;
+  walk.rows64 = rows64;
+  walk.vocab = V;
+  walk.dim = D;
+  walk.dim_kb = (D + GEMM_BK - 1) / GEMM_BK;
+  walk.dim_tiles = (D + HB_BN - 1) / HB_BN;
+  walk.piece = plan.piece;
+  walk.pieces = plan.pieces;
+  walk.split_n = plan.split_n;
+  walk.want_dx = g->dx != nullptr;
+  walk.want_dw = g->dw != nullptr;
+  walk.dw_f32 = g->dw_f32 != 0;
+  if (plan.cg == 2) NE_LAUNCH(launch_walk<2>(maps, walk, dz, plan.clusters, ctx->st));
+  else NE_LAUNCH(launch_walk<1>(maps, walk, dz, plan.clusters, ctx->st));
   if (g->dx) {
     const dim3 grid((unsigned)(((long long)rows * (D / 4) + 255) / 256));
     const long long slab = (long long)rows64 * D;
@@ -834,9 +822,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
                o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
                o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8),
                o_xp = take(R256 * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
-               o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz0 = take(dz), o_dz1 = take(dz),
+               o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz = take(HB_BUFS * dz),
                o_dx = take(std::max(up(R, 64) * D * 4, kSlabBytes)),
-               o_counters = take((up(V, HB_BN) / HB_BN + 1) * 4);
+               o_counters = take((3 * (up(V, HB_BN) / HB_BN) + 1) * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
   if (s != NE_OK) return s;
@@ -854,8 +842,7 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   n.zt = (float*)(b + o_zt);
   n.stats = (float2*)(b + o_stats);
   n.xp = (__nv_bfloat16*)(b + o_xp);
-  n.dz[0] = (__nv_bfloat16*)(b + o_dz0);
-  n.dz[1] = (__nv_bfloat16*)(b + o_dz1);
+  n.dz = (__nv_bfloat16*)(b + o_dz);
   n.dx = (float*)(b + o_dx);
   n.counters = (int*)(b + o_counters);
   ctx->head = new HeadState(n);
