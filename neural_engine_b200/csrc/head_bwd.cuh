@@ -30,7 +30,7 @@
 namespace ne {
 
 constexpr int HB_BN = 256;
-constexpr int HB_SLOTS = 4;
+constexpr int HB_SLOTS = 8;
 constexpr int HB_THREADS = GEMM_THREADS + 32;   // warps: A, MMA, 8 x epilogue, B
 constexpr int HB_BOX = 4096;                    // 32 rows of 128 bytes
 constexpr int HB_TAB = 256;                     // ids per entry of a row's index
@@ -51,20 +51,20 @@ constexpr int HB_BUFS = 3;   // pieces of dz alive: made, waited for, read
 
 struct HeadWalk {
   const int* d_rows;        // packed rows
-  int* counters;            // units drawn, then three per piece, all zero at launch
+  int* counters;            // units drawn, then head_flag's, all zero at launch
   int* status;
   int rows64;               // rows of a dz buffer and of a slab of dx
   int vocab, dim, dim_kb, dim_tiles;   // dim also in k-blocks of 64 and tiles of 256
   int piece, pieces;        // ids a piece (a multiple of 256)
-  int split_n;              // ids a split of dx's product (a multiple of 64)
+  int split_n, splits;      // ids a split of dx's product (a multiple of 256), splits a piece
   int want_dx, want_dw, dw_f32;
 };
-// counters of piece p: dz written (per epilogue warp), dz read (per unit), dx
-// added (per epilogue warp)
-enum HeadFlag : int { HF_MADE = 0, HF_READ = 1, HF_ADDED = 2 };
+// Counters of piece p: dz read (per unit), dx added (per epilogue warp), and for
+// each split of its ids dz written (per epilogue warp).
 __device__ __forceinline__ int* head_flag(const HeadWalk& s, int p, int what) {
-  return s.counters + 1 + 3 * p + what;
+  return s.counters + 1 + (2 + s.splits) * p + what;
 }
+enum HeadFlag : int { HF_READ = 0, HF_ADDED = 1, HF_MADE = 2 };   // HF_MADE + split
 
 // The sparse targets of the rows: sorted ids, [entry][row], INT_MAX behind the
 // last.
@@ -78,30 +78,46 @@ struct HeadTargets {
   int n;                       // entries a row
 };
 
+// A walk over a row's entries.  The entry behind the next one is read ahead: a
+// chunk of columns passes faster than a load arrives.
 struct TargetCursor {
-  int row, at, next;     // row of the arrays (-1: none), entry, its id
+  int row;               // of the arrays (-1: none)
+  int at;                // the next entry
+  int next, after;       // its id, and the one behind it
+  float q, q_after;      // their probabilities
 };
 
+template <bool PROB>
+__device__ __forceinline__ void cursor_load(const HeadTargets& t, const TargetCursor& c, int at, int& id,
+                                            float& q) {
+  id = 0x7fffffff;
+  q = 1.0f;
+  if (at < t.n) {
+    id = t.ids[at * t.ld + c.row];
+    if (PROB && t.prob) q = t.prob[at * t.ld + c.row];
+  }
+}
+template <bool PROB>
+__device__ __forceinline__ void cursor_step(const HeadTargets& t, TargetCursor& c) {
+  ++c.at;
+  c.next = c.after;
+  c.q = c.q_after;
+  cursor_load<PROB>(t, c, c.at + 1, c.after, c.q_after);
+}
 // The first entry of row m with an id of at least col0.  Few entries lie
 // between a multiple of 256 and col0, so they are stepped over; a search of the
 // whole row would be a chain of log2 n loads, 600 cycles each.
+template <bool PROB>
 __device__ __forceinline__ void cursor_seek(const HeadTargets& t, TargetCursor& c, int m, int rows,
                                             int col0) {
   c.row = m < rows ? (t.row_of ? t.row_of[m] : m) : -1;
   c.at = 0;
-  c.next = 0x7fffffff;
+  c.next = c.after = 0x7fffffff;
   if (c.row < 0) return;
   if (t.tab) c.at = t.tab[(long long)c.row * t.tab_ld + col0 / HB_TAB];
-  while (c.at < t.n) {
-    c.next = t.ids[c.at * t.ld + c.row];
-    if (c.next >= col0) return;
-    ++c.at;
-  }
-  c.next = 0x7fffffff;
-}
-__device__ __forceinline__ void cursor_step(const HeadTargets& t, TargetCursor& c) {
-  ++c.at;
-  c.next = c.at < t.n ? t.ids[c.at * t.ld + c.row] : 0x7fffffff;
+  cursor_load<PROB>(t, c, c.at, c.next, c.q);
+  cursor_load<PROB>(t, c, c.at + 1, c.after, c.q_after);
+  while (c.next < col0) cursor_step<PROB>(t, c);
 }
 
 // What turns logits into dz = a (2^(c2 acc - lse log2 e) - p), a = g T scale.
@@ -143,11 +159,24 @@ __device__ __forceinline__ int unit_cols(int cols, int nt) {
   return min(HB_BN, (cols - nt * HB_BN + 31) & ~31);
 }
 
-// Where the walk stands: what every role derives once from the number of rows.
+// Division by a number that does not change (d >= 1, u >= 0): the quotient by the
+// rounded-down reciprocal is short by one at most.
+struct FastDiv {
+  unsigned d, r;
+  __device__ explicit FastDiv(int by) : d(by), r(0xffffffffu / (unsigned)by) {}
+  __device__ __forceinline__ int div(int u) const {
+    unsigned q = __umulhi((unsigned)u, r);
+    if ((unsigned)u - q * d >= d) ++q;
+    return (int)q;
+  }
+};
+
+// What the walk is made of, derived once from the number of rows.
 struct HeadOrder {
-  int blocks, m_tiles, tile_m;
+  int blocks, m_tiles;
   int last_ids;              // of the last piece
   HeadCounts full, last;     // units of a whole piece and of the last one
+  FastDiv by_phase, by_m, by_d;
 };
 
 // unit u of the walk (HK_END behind the last one)
@@ -162,9 +191,9 @@ __device__ __forceinline__ void head_unit(const HeadWalk& s, const HeadOrder& o,
   } else {
     u -= made0;
     // phase q makes piece q + 1 and uses piece q; the last one makes none
-    const int phase = o.full.dz + o.full.dx + o.full.dw;
+    const int phase = (int)o.by_phase.d;
     const int whole = max(P - 2, 0);
-    int q = min(u / phase, whole);
+    int q = min(o.by_phase.div(u), whole);
     u -= q * phase;
     if (q == whole && P > 1) {
       const int n = o.last.dz + o.full.dx + o.full.dw;
@@ -188,8 +217,8 @@ __device__ __forceinline__ void head_unit(const HeadWalk& s, const HeadOrder& o,
   if (made >= 0) {
     w.kind = HK_DZ;
     w.piece = made;
-    w.mt = kind_at % o.m_tiles;
-    w.nt = kind_at / o.m_tiles;
+    w.nt = o.by_m.div(kind_at);
+    w.mt = kind_at - w.nt * o.m_tiles;
     w.kb = s.dim_kb;
     w.n = unit_cols(made == P - 1 ? o.last_ids : s.piece, w.nt);
     return;
@@ -199,17 +228,17 @@ __device__ __forceinline__ void head_unit(const HeadWalk& s, const HeadOrder& o,
   w.piece = used;
   if (u < c.dx) {
     w.kind = HK_DX;
-    w.nt = u % s.dim_tiles;
-    const int r = u / s.dim_tiles;
-    w.mt = r % o.m_tiles;
-    w.split = r / o.m_tiles;
+    const int r = o.by_d.div(u);
+    w.nt = u - r * s.dim_tiles;
+    w.split = o.by_m.div(r);
+    w.mt = r - w.split * o.m_tiles;
     w.kb0 = w.split * (s.split_n / GEMM_BK);
     w.kb = (min(ids - w.split * s.split_n, s.split_n) + GEMM_BK - 1) / GEMM_BK;
   } else if (u - c.dx < c.dw) {
     u -= c.dx;
     w.kind = HK_DW;
-    w.nt = u % s.dim_tiles;
-    w.mt = u / s.dim_tiles;
+    w.mt = o.by_d.div(u);
+    w.nt = u - w.mt * s.dim_tiles;
     w.kb = o.blocks;
   } else {
     w.kind = HK_END;
@@ -391,14 +420,12 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
   int drawn = threadIdx.x == 0 && crank == 0 ? atomicAdd(sp.counters, 1) : 0;
   // whole blocks of 64 rows, at least one (its rows are zeros)
   const int count = *sp.d_rows;
-  HeadOrder ord;
-  ord.blocks = max((count + GEMM_BK - 1) / GEMM_BK, 1);
-  ord.tile_m = TILE_M;
-  const int M = ord.blocks * GEMM_BK;
-  ord.m_tiles = (M + TILE_M - 1) / TILE_M;
-  ord.last_ids = sp.vocab - (sp.pieces - 1) * sp.piece;
-  ord.full = head_counts(sp, ord.m_tiles, TILE_M, sp.piece);
-  ord.last = head_counts(sp, ord.m_tiles, TILE_M, ord.last_ids);
+  const int blocks = max((count + GEMM_BK - 1) / GEMM_BK, 1);
+  const int M = blocks * GEMM_BK, m_tiles = (M + TILE_M - 1) / TILE_M;
+  const int last_ids = sp.vocab - (sp.pieces - 1) * sp.piece;
+  const HeadCounts full = head_counts(sp, m_tiles, TILE_M, sp.piece);
+  const HeadOrder ord{blocks, m_tiles, last_ids, full, head_counts(sp, m_tiles, TILE_M, last_ids),
+                      FastDiv(full.dz + full.dx + full.dw), FastDiv(m_tiles), FastDiv(sp.dim_tiles)};
 
   // a role other than the leader's producer takes the unit of slot `it`
   auto take = [&](int it, HeadUnit& w) -> bool {
@@ -432,29 +459,36 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       // hands over the leader's next unit once what it depends on is done: dz,
       // its buffer was read for the last time; dx and dw, dz was written, and dx
       // was added to by the piece before.  now: wait for that.
+      // What is known to be done: pieces read and added up to here, and the split
+      // written last asked for (units come in the order of pieces and kinds).
+      int read_to = -1, added_to = -1, made_piece = -1, made_split = -1;
+      auto reached = [&](int* f, int want, bool now) -> bool {
+        if (flag_reached(f, want)) return true;
+        if (now && !flag_wait(f, want, sp.status, abort_flag)) ok = false;
+        return now && ok;
+      };
       auto hand_over = [&](int it, bool now) -> bool {
-        const int* f[2] = {nullptr, nullptr};
-        int want[2] = {0, 0};
         if (nw.kind == HK_DZ) {
-          if (nw.piece >= HB_BUFS) {
-            f[0] = head_flag(sp, nw.piece - HB_BUFS, HF_READ);
-            want[0] = ord.full.dx + ord.full.dw;
+          const int p = nw.piece - HB_BUFS;
+          if (p > read_to) {
+            if (!reached(head_flag(sp, p, HF_READ), ord.full.dx + ord.full.dw, now)) return false;
+            read_to = p;
           }
         } else if (nw.kind != HK_END) {
-          f[0] = head_flag(sp, nw.piece, HF_MADE);
-          want[0] = (nw.piece == sp.pieces - 1 ? ord.last.dz : ord.full.dz) * CG * GEMM_EPI_WARPS;
-          if (nw.kind == HK_DX && nw.piece > 0) {
-            f[1] = head_flag(sp, nw.piece - 1, HF_ADDED);
-            want[1] = ord.full.dx * CG * GEMM_EPI_WARPS;
+          const int split = nw.kind == HK_DX ? nw.split : nw.mt * TILE_M / sp.split_n;
+          if (nw.piece != made_piece || split != made_split) {
+            const int ids = nw.piece == sp.pieces - 1 ? ord.last_ids : sp.piece;
+            const int n = (min(ids - split * sp.split_n, sp.split_n) + HB_BN - 1) / HB_BN;
+            if (!reached(head_flag(sp, nw.piece, HF_MADE + split),
+                         n * ord.m_tiles * CG * GEMM_EPI_WARPS, now))
+              return false;
+            made_piece = nw.piece;
+            made_split = split;
           }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!f[i] || flag_reached(f[i], want[i])) continue;
-          if (!now) return false;
-          if (!flag_wait(f[i], want[i], sp.status, abort_flag)) {
-            ok = false;
-            return false;
+          if (nw.kind == HK_DX && nw.piece - 1 > added_to) {
+            if (!reached(head_flag(sp, nw.piece - 1, HF_ADDED), ord.full.dx * CG * GEMM_EPI_WARPS, now))
+              return false;
+            added_to = nw.piece - 1;
           }
         }
         const int s = it % HB_SLOTS;
@@ -469,8 +503,14 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         if constexpr (PAIR) post_unit(mapa_shared(at, 1), mapa_shared(sfull_bar + 8 * s, 1), nw);
         return true;
       };
-      if (leads) {
+      // draws the unit after the one drawn before; the latency of the counter
+      // passes behind a unit's loads
+      auto next_unit = [&] {
         head_unit(sp, ord, drawn, nw);
+        if (nw.kind != HK_END) drawn = atomicAdd(sp.counters, 1);
+      };
+      if (leads) {
+        next_unit();
         hand_over(0, true);
       }
       for (int it = 0; ok; ++it) {
@@ -478,7 +518,6 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         bool handed = false;
         if (leads) {
           w = nw;
-          if (w.kind != HK_END) drawn = atomicAdd(sp.counters, 1);   // arrives behind the loads
         } else {
           if (!take(it, w)) break;
           taken(it);
@@ -517,13 +556,13 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           if (leads && k == 1) {   // the loads are ahead of the MMAs now: time for the next unit
-            head_unit(sp, ord, drawn, nw);
+            next_unit();
             handed = hand_over(it + 1, false);
             if (!ok) break;
           }
         }
         if (leads && ok && !handed) {
-          if (w.kb < 2) head_unit(sp, ord, drawn, nw);
+          if (w.kb < 2) next_unit();
           hand_over(it + 1, true);
         }
       }
@@ -633,7 +672,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
           keep = 0xffffffffu;
           sign = co.x < 0.f ? 0x80008000u : 0u;
         }
-        cursor_seek(dzp.t, cur, m, count, id0 + n_tile + 128 * half);
+        cursor_seek<true>(dzp.t, cur, m, count, id0 + n_tile + 128 * half);
       }
       if (lane == 0 && owed && !mbar_try_wait(tfull_bar + 8 * acc, acc_phase)) settle();
       const bool ready = mbar_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag);
@@ -677,12 +716,11 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
               while (cur.next < col + 32) {
                 if (cur.next >= col) {
                   const int j = cur.next - col;
-                  const float q = dzp.t.prob ? dzp.t.prob[cur.at * dzp.t.ld + cur.row] : 1.0f;
 #pragma unroll
                   for (int i = 0; i < 32; ++i)
-                    if (i == j) v[i] -= mag * q;
+                    if (i == j) v[i] -= mag * cur.q;
                 }
-                cursor_step(dzp.t, cur);
+                cursor_step<true>(dzp.t, cur);
               }
             }
             // rounded once to bf16: dz is the operand of two tensor-core
@@ -723,7 +761,8 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         // others wait for what this unit wrote
         if (w.kind != HK_DW) {
           if (owed) settle();   // a unit without a box of its own
-          owed = head_flag(sp, w.piece, w.kind == HK_DZ ? HF_MADE : HF_ADDED);
+          owed = head_flag(sp, w.piece,
+                           w.kind == HK_DZ ? HF_MADE + w.nt * HB_BN / sp.split_n : HF_ADDED);
         }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }

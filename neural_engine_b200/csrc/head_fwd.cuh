@@ -197,7 +197,7 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
       const int m = mt * TILE_M + lane_row;
       const int n_tile = nt * p.bn, n_end = min(n_tile + p.bn, p.vocab);
       TargetCursor cur;
-      cursor_seek(p.t, cur, m, M, n_tile);
+      cursor_seek<false>(p.t, cur, m, M, n_tile);
       if (!p.one_row_tile) {
         mx = lowest;
         sum = 0.f;
@@ -238,7 +238,7 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
                 if (i == j) z = v[i];
               p.zt[cur.at * p.t.ld + cur.row] = z * p.c2;
             }
-            cursor_step(p.t, cur);
+            cursor_step<false>(p.t, cur);
           }
         }
         if (!p.one_row_tile && cur.row >= 0)

@@ -174,118 +174,69 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
   }
 }
 
-// One warp per row: the softmax over the row's entries, then its ids sorted
-// with repeats added together (in the order of the entries), K^2 comparisons
-// out of shared memory, and an index: how many ids are below each multiple of
-// 256.
-constexpr int TEACHER_WARPS = 4;
-__global__ void __launch_bounds__(32 * TEACHER_WARPS) head_teacher_kernel(
+// One block per row, one thread per entry: the softmax over the row's entries,
+// the ids sorted (each entry counts those that go before it, out of shared
+// memory; equal ids keep their order and stand beside each other, each with its
+// probability), and an index: how many ids are below each multiple of 256.
+template <bool MAX>
+__device__ __forceinline__ float block_reduce(float v, float* part, int warps) {
+  v = MAX ? warp_max(v) : warp_sum(v);
+  __syncthreads();   // the last use of `part`
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = part[0];
+  for (int w = 1; w < warps; ++w) v = MAX ? fmaxf(v, part[w]) : v + part[w];
+  return v;
+}
+__global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
     const int32_t* __restrict__ ids_in, const float* __restrict__ logit, int rows, int K, int vocab,
     float inv_t, int* ids, float* prob, unsigned short* tab, int tab_ld, float* neg_entropy,
     int* keep, int* status) {
   pdl_trigger();
   pdl_wait();
-  __shared__ __align__(16) int sid[TEACHER_WARPS][kTopkMax];
-  __shared__ __align__(16) float sp[TEACHER_WARPS][kTopkMax];
-  __shared__ __align__(16) int sfirst[TEACHER_WARPS][kTopkMax];
-  __shared__ int sorted[TEACHER_WARPS][kTopkMax];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.x * TEACHER_WARPS + w;
-  if (r >= rows) return;
-  const int32_t* id = ids_in + (long long)r * K;
-  const float* y = logit + (long long)r * K;
-  float top = -INFINITY;
-  int any = 0;
-  for (int k = lane; k < K; k += 32) {
-    int c = id[k];
+  __shared__ __align__(16) unsigned sid[kTopkMax];
+  __shared__ unsigned sorted[kTopkMax];
+  __shared__ float part[kTopkMax / 32];
+  const int r = blockIdx.x, k = threadIdx.x, warps = blockDim.x >> 5;
+  int c = -1;
+  float v = -INFINITY;
+  if (k < K) {
+    c = ids_in[(long long)r * K + k];
+    v = logit[(long long)r * K + k] * inv_t;
     if (c >= vocab) atomicExch(status, DEV_ERR_BOUNDS);
-    const float v = y[k] * inv_t;
-    if (c < 0 || c >= vocab || v == -INFINITY) c = INT_MAX;
-    sid[w][k] = c;
-    sp[w][k] = v;
-    if (c != INT_MAX) {
-      any = 1;
-      top = fmaxf(top, v);
-    }
   }
-  any = __any_sync(0xffffffffu, any);
-  top = warp_max(top);
-  __syncwarp();
-  float sum = 0.f;
-  for (int k = lane; k < K; k += 32)
-    if (sid[w][k] != INT_MAX) sum += expf(sp[w][k] - top);
-  sum = warp_sum(sum);
-  const float lsum = logf(sum);
-  float ent = 0.f;
-  for (int k = lane; k < K; k += 32) {
-    float p = 0.f;
-    if (sid[w][k] != INT_MAX) {
-      const float l = sp[w][k] - top;
-      p = expf(l) / sum;
-      if (p != 0.f) ent += p * (l - lsum);
-    }
-    sp[w][k] = p;
-  }
-  ent = warp_sum(ent);
-  __syncwarp();
-  // the entries up to a multiple of four are absent ones
-  const int K4 = (K + 3) & ~3;
-  if (lane < K4 - K) {
-    sid[w][K + lane] = INT_MAX;
-    sp[w][K + lane] = 0.f;
-    sfirst[w][K + lane] = INT_MAX;
-  }
-  for (int k = lane; k < K; k += 32) {
-    const int c = sid[w][k];
-    int same = 0;   // an entry before it has the same id
+  const bool there = c >= 0 && c < vocab && v != -INFINITY;
+  if (!there) c = INT_MAX;
+  sid[k] = (unsigned)c;
+  const int any = __syncthreads_or(there);
+  const float top = block_reduce<true>(there ? v : -INFINITY, part, warps);
+  const float e = there ? expf(v - top) : 0.f;
+  const float sum = block_reduce<false>(e, part, warps);
+  const float p = there ? e / sum : 0.f;
+  const float ent = block_reduce<false>(there && p != 0.f ? p * (v - top - logf(sum)) : 0.f, part, warps);
+  int rank = 0;
 #pragma unroll 4
-    for (int j = 0; j < K4; j += 4) {
-      const int4 q = *reinterpret_cast<const int4*>(&sid[w][j]);
-      same |= (q.x == c && j < k) | (q.y == c && j + 1 < k) | (q.z == c && j + 2 < k) |
-              (q.w == c && j + 3 < k);
-    }
-    sfirst[w][k] = same ? INT_MAX : c;   // the id where it stands first
+  for (int j = 0; j < (int)blockDim.x; j += 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(&sid[j]);
+    rank += (q.x < (unsigned)c + (j < k)) + (q.y < (unsigned)c + (j + 1 < k)) +
+            (q.z < (unsigned)c + (j + 2 < k)) + (q.w < (unsigned)c + (j + 3 < k));
   }
-  __syncwarp();
-  int total = 0;
-  for (int k = lane; k < K; k += 32) total += sfirst[w][k] != INT_MAX;
-  total = __reduce_add_sync(0xffffffffu, total);
-  for (int k = lane; k < K; k += 32) {
-    const int c = sfirst[w][k];
-    if (c != INT_MAX) {
-      int rank = 0;
-      float p = 0.f;
-#pragma unroll 4
-      for (int j = 0; j < K4; j += 4) {
-        const int4 f = *reinterpret_cast<const int4*>(&sfirst[w][j]);
-        const int4 q = *reinterpret_cast<const int4*>(&sid[w][j]);
-        const float4 y4 = *reinterpret_cast<const float4*>(&sp[w][j]);
-        rank += (f.x < c) + (f.y < c) + (f.z < c) + (f.w < c);
-        p += q.x == c ? y4.x : 0.f;
-        p += q.y == c ? y4.y : 0.f;
-        p += q.z == c ? y4.z : 0.f;
-        p += q.w == c ? y4.w : 0.f;
-      }
-      ids[(long long)rank * rows + r] = c;
-      prob[(long long)rank * rows + r] = p;
-      sorted[w][rank] = c;
-    }
-    if (k >= total) {
-      ids[(long long)k * rows + r] = INT_MAX;
-      prob[(long long)k * rows + r] = 0.f;
-    }
+  sorted[rank] = (unsigned)c;
+  if (rank < K) {
+    ids[(long long)rank * rows + r] = c;
+    prob[(long long)rank * rows + r] = p;
   }
-  __syncwarp();
-  for (int t = lane; t < tab_ld; t += 32) {
-    int lo = 0, hi = total;
+  __syncthreads();
+  for (int t = k; t < tab_ld; t += blockDim.x) {
+    int lo = 0, hi = K;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (sorted[w][mid] < t * HB_TAB) lo = mid + 1;
+      if (sorted[mid] < (unsigned)t * HB_TAB) lo = mid + 1;
       else hi = mid;
     }
     tab[(long long)r * tab_ld + t] = (unsigned short)lo;
   }
-  if (lane == 0) {
+  if (k == 0) {
     keep[r] = any;
     neg_entropy[r] = ent;
   }
@@ -509,8 +460,7 @@ ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
   if (!c.teacher) return NE_OK;
   HeadState* h = ctx->head;
   const int rows = c.d->rows;
-  NE_LAUNCH(launch_k(head_teacher_kernel, dim3((rows + TEACHER_WARPS - 1) / TEACHER_WARPS),
-                     dim3(32 * TEACHER_WARPS), 0, ctx->st, c.teacher->ids, c.teacher->logits, rows,
+  NE_LAUNCH(launch_k(head_teacher_kernel, dim3(rows), dim3((unsigned)up(c.n, 32)), 0, ctx->st, c.teacher->ids, c.teacher->logits, rows,
                      c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->tab, tab_entries(c.d->vocab),
                      h->neg_entropy, h->keep, ctx->d_status));
   return NE_OK;
@@ -652,16 +602,18 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
   p.piece = (int)up((vocab + p.pieces - 1) / p.pieces, HB_BN);
   p.pieces = (vocab + p.piece - 1) / p.piece;
   // dx's units are the longest: where there are few of them the piece is split
-  // until a unit is a third of what a pair has to do for dx and dw (rows that do
-  // not count make that less than it looks from here), but not below 32
-  // k-blocks, twice what a unit's own hand-over and epilogue cost
+  // until a unit is two thirds of what a pair has to do for dx and dw (rows that
+  // do not count make that less than it looks from here), but not below 32
+  // k-blocks, twice what a unit's own hand-over and epilogue cost.  dw's units
+  // cost 9 k-blocks at least, their epilogue.
   const double m_tiles = (double)((rows + p.tile_m - 1) / p.tile_m), d_tiles = (dim + HB_BN - 1) / HB_BN;
   const double piece_kb = p.piece / GEMM_BK;
-  const double load = m_tiles * d_tiles * piece_kb + (p.piece / p.tile_m) * d_tiles * (double)(rows64 / GEMM_BK);
-  const double most = std::max(32.0, load / p.clusters / 3);
+  const double load = m_tiles * d_tiles * piece_kb +
+                      (p.piece / p.tile_m) * d_tiles * std::max(9.0, (double)(rows64 / GEMM_BK));
+  const double most = std::max(32.0, load / p.clusters / 1.5);
   const long long slabs = std::max<long long>(1, (long long)kSlabBytes / (rows64 * dim * 4));
   const long long want = std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
-  p.split_n = (int)up((p.piece + want - 1) / want, GEMM_BK);
+  p.split_n = (int)up((p.piece + want - 1) / want, HB_BN);
   p.splits = (p.piece + p.split_n - 1) / p.split_n;
   return p;
 }
@@ -688,7 +640,7 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   const HeadPlan plan = head_plan(rows, D, V, ctx->num_sms);
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK ||
-      (s = enqueue_pack(ctx, c, lse, grad, 1 + 3 * plan.pieces)) != NE_OK)
+      (s = enqueue_pack(ctx, c, lse, grad, 1 + plan.pieces * (2 + plan.splits))) != NE_OK)
     return s;
   HeadDz dz{};
   dz.t = targets_of(h, c, true);
@@ -722,6 +674,7 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   walk.piece = plan.piece;
   walk.pieces = plan.pieces;
   walk.split_n = plan.split_n;
+  walk.splits = plan.splits;
   walk.want_dx = g->dx != nullptr;
   walk.want_dw = g->dw != nullptr;
   walk.dw_f32 = g->dw_f32 != 0;
@@ -824,7 +777,7 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
                o_xp = take(R256 * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
                o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz = take(HB_BUFS * dz),
                o_dx = take(std::max(up(R, 64) * D * 4, kSlabBytes)),
-               o_counters = take((3 * (up(V, HB_BN) / HB_BN) + 1) * 4);
+               o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1) * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
   if (s != NE_OK) return s;
