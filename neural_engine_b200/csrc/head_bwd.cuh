@@ -57,6 +57,7 @@ struct HeadWalk {
   int vocab, dim, dim_kb, dim_tiles;   // dim also in k-blocks of 64 and tiles of 256
   int piece, pieces;        // ids a piece (a multiple of 256)
   int split_n, splits;      // ids a split of dx's product (a multiple of 256), splits a piece
+  int own_slabs;            // dx of each piece goes to slabs of its own, else they add up
   int want_dx, want_dw, dw_f32;
 };
 // Counters of piece p: dz read (per unit), dx added (per epilogue warp), and for
@@ -485,7 +486,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
             made_piece = nw.piece;
             made_split = split;
           }
-          if (nw.kind == HK_DX && nw.piece - 1 > added_to) {
+          if (nw.kind == HK_DX && !sp.own_slabs && nw.piece - 1 > added_to) {
             if (!reached(head_flag(sp, nw.piece - 1, HF_ADDED), ord.full.dx * CG * GEMM_EPI_WARPS, now))
               return false;
             added_to = nw.piece - 1;
@@ -691,8 +692,8 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       // a warp owns half of the tile's columns and sends boxes of 128-byte rows:
       // 64 columns of bf16 or 32 of fp32 at a time
       const int step = b16 ? 64 : 32;
-      const bool add = w.kind == HK_DX ? w.piece > 0 : w.kind == HK_DW && sp.dw_f32;
-      const int y = y0 + (w.kind == HK_DX ? w.split * sp.rows64
+      const bool add = w.kind == HK_DX ? w.piece > 0 && !sp.own_slabs : w.kind == HK_DW && sp.dw_f32;
+      const int y = y0 + (w.kind == HK_DX ? (w.split + (sp.own_slabs ? w.piece * sp.splits : 0)) * sp.rows64
                           : w.kind == HK_DW ? id0 : (w.piece % HB_BUFS) * sp.rows64);
 #pragma unroll 1
       for (int c = 128 * half; c < 128 * half + 128; c += step) {

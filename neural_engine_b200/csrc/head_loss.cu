@@ -508,10 +508,10 @@ HeadTargets targets_of(const HeadState* h, const HeadCall& c, bool packed) {
   return t;
 }
 
-template <int CG>
+template <int CG, bool LONG>
 cudaError_t launch_lse(const CUtensorMap& x, const CUtensorMap& w, const HeadLse& p,
                        const LsePlan& plan, long long units, cudaStream_t st) {
-  auto kern = head_lse_kernel<CG>;
+  auto kern = head_lse_kernel<CG, LONG>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan.smem);
   if (e != cudaSuccess) return e;
   const int grid = CG * (int)std::min<long long>(units, plan.clusters);
@@ -555,8 +555,11 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   if (!make_tmap(&x, plan.packed ? h->xp : d.x, rows, D, plan.packed ? (long long)up(D, GEMM_BK) : d.ldx, plan.a_rows, 0) ||
       !make_tmap(&w, d.w, V, D, d.ldw, plan.bn / plan.cg, 0))
     return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
-  if (plan.cg == 2) NE_LAUNCH(launch_lse<2>(x, w, p, plan, units, ctx->st));
-  else NE_LAUNCH(launch_lse<1>(x, w, p, plan, units, ctx->st));
+  const bool lng = p.dim_kb > HF_LONG_FROM;   // long sums (head_fwd.cuh)
+  if (plan.cg == 2 && lng) NE_LAUNCH((launch_lse<2, true>(x, w, p, plan, units, ctx->st)));
+  else if (plan.cg == 2) NE_LAUNCH((launch_lse<2, false>(x, w, p, plan, units, ctx->st)));
+  else if (lng) NE_LAUNCH((launch_lse<1, true>(x, w, p, plan, units, ctx->st)));
+  else NE_LAUNCH((launch_lse<1, false>(x, w, p, plan, units, ctx->st)));
   HeadJoin j{};
   j.stats = h->stats;
   j.part_stride = p.part_stride;
@@ -588,6 +591,7 @@ struct HeadPlan {
   int cg, tile_m, clusters;   // CTAs a tile, rows a tile, clusters at once
   int piece, pieces;          // ids a piece (whole tiles), pieces
   int split_n, splits;        // ids a split of dx's product
+  bool own_slabs;             // pieces do not add up into the same slabs
 };
 
 HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
@@ -615,6 +619,8 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
   const long long want = std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
   p.split_n = (int)up((p.piece + want - 1) / want, HB_BN);
   p.splits = (p.piece + p.split_n - 1) / p.split_n;
+  // with room for it, no piece's dx waits for the piece before
+  p.own_slabs = (long long)p.splits * p.pieces <= slabs;
   return p;
 }
 
@@ -655,7 +661,8 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
             make_tmap_out(&maps.dz_out, h->dz, dz_rows, plan.piece, plan.piece, bf, 2, 64) &&
             make_tmap(&maps.dz_k, h->dz, dz_rows, plan.piece, plan.piece, GEMM_BM, 0) &&
             make_tmap_mn(&maps.w_mn, d.w, D, V, d.ldw) &&
-            make_tmap_out(&maps.dx_out, h->dx, plan.splits * rows64, D, D, f32, 4, 32) &&
+            make_tmap_out(&maps.dx_out, h->dx, plan.splits * (plan.own_slabs ? plan.pieces : 1) * rows64,
+                          D, D, f32, 4, 32) &&
             make_tmap_mn(&maps.dz_mn, h->dz, plan.piece, dz_rows, plan.piece) &&
             make_tmap_mn(&maps.x_mn, h->xp, D, rows64, ldp);
   maps.dw_out = maps.dx_out;   // not used without dw
@@ -675,6 +682,7 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   walk.pieces = plan.pieces;
   walk.split_n = plan.split_n;
   walk.splits = plan.splits;
+  walk.own_slabs = plan.own_slabs;
   walk.want_dx = g->dx != nullptr;
   walk.want_dw = g->dw != nullptr;
   walk.dw_f32 = g->dw_f32 != 0;
@@ -683,7 +691,11 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   if (g->dx) {
     const dim3 grid((unsigned)(((long long)rows * (D / 4) + 255) / 256));
     const long long slab = (long long)rows64 * D;
-    const int slabs = (std::min(plan.piece, V) + plan.split_n - 1) / plan.split_n;
+    // the last piece may have fewer splits than the others
+    const int last = V - (plan.pieces - 1) * plan.piece;
+    const int slabs = !plan.own_slabs && plan.pieces > 1
+                          ? plan.splits
+                          : (plan.pieces - 1) * plan.splits + (last + plan.split_n - 1) / plan.split_n;
     if (g->dx_f32)
       NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
                          slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx));

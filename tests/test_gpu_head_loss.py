@@ -191,6 +191,21 @@ def test_large_logits(eng):
     h.run(eng).check()
 
 
+@pytest.mark.parametrize("rows", [3, 200, 600])
+def test_long_sums(eng, rows):
+    """Dims beyond 2048, whole and not in the lengths the sum is taken in: the
+    bound's term per column is held to 1536 of them there."""
+    for dim in (2056, 4096):
+        h = Head(rows, dim, 520, seed=dim).ce(0.1).run(eng)
+        h.check()
+        keep, p, plogp = h.targets()
+        want = oh.head_loss(h.x, h.w, keep, p, plogp)
+        # 4.8e-10 a column of 1536, and of the other roundings 2^-22 each of the
+        # logits' sum, its logarithm and the change of base
+        size = float(want[1].abs().max())
+        assert float((h.lse[:rows].cpu().double() - want[1]).abs().max()) <= (1536 * 4.8e-10 + 3 * 2.0 ** -22) * size
+
+
 def test_teacher_entries(eng):
     """Repeats, -inf, ids in any order, NaN and infinity behind absent ids, 256 entries."""
     h = Head(6, 64, 90, seed=5).distill(256, 1.0, ragged=False)
