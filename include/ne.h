@@ -455,6 +455,17 @@ NE_API ne_status ne_head_distill_bwd(ne_ctx* ctx, const ne_head_desc* d, const n
                                      const float* d_lse, const float* d_grad,
                                      const ne_head_grads* g);
 
+/* The classifier stage of a micro-step (the per-layer entry points above) with a
+ * teacher: takes the place of ne_lmhead_ce_fwd_bwd.  Row i of `t` belongs to
+ * target i of the batch ([B][S] order); the row's loss is (1 - hard_weight)
+ * times its distillation loss plus hard_weight times its cross entropy, the
+ * batch's the mean over the B*S rows (a row without entries adds 0 to the
+ * first).  hard_weight is 0 .. 1; with 1 `t` may be NULL, which is the cross
+ * entropy of ne_lmhead_ce_fwd_bwd without its logits.  Needs ne_head_alloc for
+ * B*S rows and the model's dim and vocab, and no vocabulary map. */
+NE_API ne_status ne_lmhead_distill_fwd_bwd(ne_ctx* ctx, const ne_teacher_desc* t, float hard_weight,
+                                           float* d_loss);
+
 /* ---- data-parallel gradients (NCCL over NVLink; no reference counterpart:
  * the reference trains on one device) ---------------------------------------
  * Rank 0 makes an id with ne_comm_unique_id and shares it out of band; every

@@ -55,6 +55,7 @@ struct HeadState {
   float* prob = nullptr;          // [topk][rows]
   float* neg_entropy = nullptr;   // [rows] sum p log p
   float* zt = nullptr;            // [topk][rows] target logits, log2 units
+  float* lse = nullptr;           // [rows] between the passes of head_train
   float2* stats = nullptr;        // (max, sum exp2) of each row and half tile
   __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim up to 64] packed x
   __nv_bfloat16* dz = nullptr;    // [3][rows up to 64][piece]
@@ -105,7 +106,7 @@ struct HeadPack {
   // backward
   const float* lse;
   const float* grad;        // NULL: ones
-  float factor;             // T * scale
+  float factor;             // T * scale (* the loss's weight)
   float2* coef;             // NULL: forward
   int* counters;
   int n_counters;
@@ -257,6 +258,8 @@ struct HeadJoin {
   const float* neg_entropy;
   const float* zt;
   float t2;                       // T^2
+  float weight;
+  int add;                        // to loss
   float* loss;
   float* lse;
   int* status;
@@ -328,7 +331,8 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
     } else if (on) {
       loss = kLn2 * (lse2 - p.zt[m]);
     }
-    p.loss[i] = loss;
+    loss *= p.weight;
+    p.loss[i] = p.add ? p.loss[i] + loss : loss;
     p.lse[i] = on ? kLn2 * lse2 : 0.f;
   }
 }
@@ -339,7 +343,7 @@ template <class T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int slabs,
                                                       long long slab, int rows, int dim,
                                                       const int* __restrict__ pos_of, T* dx,
-                                                      long long ld) {
+                                                      long long ld, int add) {
   pdl_trigger();
   pdl_wait();
   const int quads = dim / 4;
@@ -358,6 +362,10 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
   }
   T* dst = dx + (long long)i * ld + 4 * k;
   if constexpr (sizeof(T) == 4) {
+    if (add) {
+      const float4 q = *reinterpret_cast<const float4*>(dst);
+      v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+    }
     *reinterpret_cast<float4*>(dst) = v;
   } else {
     uint2 o;
@@ -422,6 +430,8 @@ struct HeadCall {
   const ne_teacher_desc* teacher = nullptr;
   float t = 1.0f;
   int n = 1;
+  float weight = 1.0f;                  // of the loss and its gradient
+  bool add = false;                     // to loss and dx
 };
 
 ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
@@ -486,7 +496,7 @@ ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, const float* lse, const f
   p.ldp = (long long)up(p.dim, GEMM_BK);
   p.lse = lse;
   p.grad = grad;
-  p.factor = c.t * c.d->scale;
+  p.factor = c.t * c.d->scale * c.weight;
   p.coef = lse ? h->coef : nullptr;
   p.counters = h->counters;
   p.n_counters = counters;
@@ -576,6 +586,8 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   j.neg_entropy = h->neg_entropy;
   j.zt = h->zt;
   j.t2 = c.t * c.t;
+  j.weight = c.weight;
+  j.add = c.add;
   j.loss = loss;
   j.lse = lse;
   j.status = ctx->d_status;
@@ -698,11 +710,11 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
                           : (plan.pieces - 1) * plan.splits + (last + plan.split_n - 1) / plan.split_n;
     if (g->dx_f32)
       NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
-                         slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx));
+                         slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx, (int)c.add));
     else
       NE_LAUNCH(launch_k(head_dx_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->st,
                          (const float*)h->dx, slabs, slab, rows, D, (const int*)h->pos_of,
-                         (__nv_bfloat16*)g->dx, g->lddx));
+                         (__nv_bfloat16*)g->dx, g->lddx, 0));
   }
   return NE_OK;
 }
@@ -726,6 +738,31 @@ ne_status no_rows(ne_ctx* ctx, const ne_head_desc* d, const ne_head_grads* g) {
 }
 
 }  // namespace
+
+ne_status head_train(ne_ctx* ctx, const ne_head_desc* d, const int32_t* target,
+                     const ne_teacher_desc* teacher, float hard, float weight, float* loss, float* dx,
+                     float* dw) {
+  const char* what = "ne_lmhead_distill_fwd_bwd";
+  ne_status s = head_check(ctx, d, what);
+  if (s != NE_OK || (teacher && (s = teacher_check(ctx, teacher, what)) != NE_OK)) return s;
+  const ne_head_grads g{dx, d->dim, 1, dw, d->dim, 1};
+  HeadCall c;
+  c.d = d;
+  for (int part = 0; part < 2; ++part) {
+    const float share = part == 0 ? 1.0f - hard : hard;
+    if (share == 0.f) continue;
+    c.teacher = part == 0 ? teacher : nullptr;
+    c.target = part == 0 ? nullptr : target;
+    c.t = c.teacher ? teacher->temperature : 1.0f;
+    c.n = c.teacher ? teacher->topk : 1;
+    c.weight = share;
+    if ((s = head_forward(ctx, c, loss, ctx->head->lse)) != NE_OK) return s;
+    c.weight = share * weight;
+    if ((s = head_backward(ctx, c, ctx->head->lse, nullptr, &g)) != NE_OK) return s;
+    c.add = true;
+  }
+  return NE_OK;
+}
 
 void free_head(ne_ctx* ctx) {
   if (!ctx->head) return;
@@ -785,7 +822,7 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   };
   const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4),
                o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
-               o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8),
+               o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8), o_lse = take(R * 4),
                o_xp = take(R256 * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
                o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz = take(HB_BUFS * dz),
                o_dx = take(std::max(up(R, 64) * D * 4, kSlabBytes)),
@@ -806,6 +843,7 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   n.neg_entropy = (float*)(b + o_ent);
   n.zt = (float*)(b + o_zt);
   n.stats = (float2*)(b + o_stats);
+  n.lse = (float*)(b + o_lse);
   n.xp = (__nv_bfloat16*)(b + o_xp);
   n.dz = (__nv_bfloat16*)(b + o_dz);
   n.dx = (float*)(b + o_dx);

@@ -22,6 +22,12 @@ struct Comm;                            // comm.cu
 void comm_free(ne_ctx* ctx);            // comm.cu
 struct HeadState;                       // head_loss.cu
 void free_head(ne_ctx* ctx);            // head_loss.cu
+// (1 - hard) * distillation + hard * cross entropy of the rows of d: row losses
+// (written), dx (written) and dw (added to) of `weight` times their sum, fp32.
+// teacher may be NULL where hard is 1.
+ne_status head_train(ne_ctx* ctx, const ne_head_desc* d, const int32_t* target,
+                     const ne_teacher_desc* teacher, float hard, float weight, float* loss, float* dx,
+                     float* dw);        // head_loss.cu
 }  // namespace ne
 
 namespace ne {

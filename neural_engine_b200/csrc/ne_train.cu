@@ -1212,6 +1212,23 @@ NE_API ne_status ne_ffn_fwd(ne_ctx* ctx, int l) {
   return NE_OK;
 }
 
+// What follows the classifier's gradients: the final RMSNorm's backward (dY for
+// the last layer), the batch's mean loss and the gradient exchange.
+static ne_status after_classifier(ne_ctx* ctx, float* d_loss) {
+  NE_TRAIN_PRELUDE();
+  NE_LAUNCH(launch_rmsnorm_bwd(t->dXF, t->XL, ctx->rms_final, m.rms_eps, M, D, nullptr, t->dY,
+                               t->dY16, t->rmsf_g, st));
+  if (d_loss) {
+    NE_CUDA(cudaMemsetAsync(t->red + 1, 0, sizeof(double), st));
+    sum_rows_kernel<<<64, 256, 0, st>>>(t->loss_rows, M, t->red + 1);
+    NE_CUDA(cudaGetLastError());
+    // d_loss = sum / M  (a 1-thread kernel keeps it on the device)
+    mean_from_sum_kernel<<<1, 1, 0, st>>>(t->red + 1, M, d_loss);
+    NE_CUDA(cudaGetLastError());
+  }
+  return comm_after_lmhead(ctx);
+}
+
 // Classifier over the tied embedding (train.m:495-505), mean cross-entropy
 // (cpu_ops.h:348-382), the classifier's backward (dX and the dense part of
 // dE), and the final RMSNorm's backward, leaving dY for the last layer.
@@ -1247,17 +1264,25 @@ NE_API ne_status ne_lmhead_ce_fwd_bwd(ne_ctx* ctx, float* d_loss) {
       return s;
   }
   if (cmp) NE_LAUNCH(launch_scatter_add_rows(t->dEc, t->d_c2f, t->CV, D, t->embed_g, st));
-  NE_LAUNCH(launch_rmsnorm_bwd(t->dXF, t->XL, ctx->rms_final, m.rms_eps, M, D, nullptr, t->dY,
-                               t->dY16, t->rmsf_g, st));
-  if (d_loss) {
-    NE_CUDA(cudaMemsetAsync(t->red + 1, 0, sizeof(double), st));
-    sum_rows_kernel<<<64, 256, 0, st>>>(t->loss_rows, M, t->red + 1);
-    NE_CUDA(cudaGetLastError());
-    // d_loss = sum / M  (a 1-thread kernel keeps it on the device)
-    mean_from_sum_kernel<<<1, 1, 0, st>>>(t->red + 1, M, d_loss);
-    NE_CUDA(cudaGetLastError());
-  }
-  return comm_after_lmhead(ctx);
+  return after_classifier(ctx, d_loss);
+}
+
+// The classifier stage of a micro-step with a teacher's top logits in place of,
+// or beside, the hard targets (ne.h); the logits are not kept.
+NE_API ne_status ne_lmhead_distill_fwd_bwd(ne_ctx* ctx, const ne_teacher_desc* teacher,
+                                           float hard_weight, float* d_loss) {
+  NE_TRAIN_PRELUDE();
+  if (!(hard_weight >= 0.f && hard_weight <= 1.f))
+    return fail(ctx, NE_ERR_INVALID, "ne_lmhead_distill_fwd_bwd: hard_weight is between 0 and 1");
+  if (!teacher && hard_weight != 1.f)
+    return fail(ctx, NE_ERR_INVALID, "ne_lmhead_distill_fwd_bwd: teacher is NULL");
+  if (t->CV > 0)
+    return fail(ctx, NE_ERR_STATE, "ne_lmhead_distill_fwd_bwd: a vocabulary map is set");
+  const ne_head_desc d{t->XNF, D, ctx->embed, D, M, D, V, 1.0f};
+  if ((s = head_train(ctx, &d, t->tgt, teacher, hard_weight, 1.0f / (float)M, t->loss_rows, t->dXF,
+                      t->embed_g)) != NE_OK)
+    return s;
+  return after_classifier(ctx, d_loss);
 }
 
 // FFN backward of a layer (ffnBwdFull, mil_dynamic.h:320-409): d_gate -> dh1,

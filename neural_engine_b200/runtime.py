@@ -39,7 +39,7 @@ EXPORTED = ("ne_init", "ne_free", "ne_last_error", "ne_status_str", "ne_sync", "
             "ne_train_value_ranges", "ne_comm_set_timeout", "ne_shard_range",
             "ne_gemm_dw_owned", "ne_ckpt_probe", "ne_fault_calls",
             "ne_head_alloc", "ne_head_ce_fwd", "ne_head_ce_bwd", "ne_head_distill_fwd",
-            "ne_head_distill_bwd")
+            "ne_head_distill_bwd", "ne_lmhead_distill_fwd_bwd")
 
 def shard_range(n: int, world: int, rank: int, lib=None):
     """(offset, length) of the part of an n-element tensor that `rank` owns
@@ -251,6 +251,7 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
     lib.ne_head_ce_bwd.argtypes = [P, H, P, P, P, G]
     lib.ne_head_distill_fwd.argtypes = [P, H, T, P, P]
     lib.ne_head_distill_bwd.argtypes = [P, H, T, P, P, G]
+    lib.ne_lmhead_distill_fwd_bwd.argtypes = [P, T, F, P]
     lib.ne_stream_read.argtypes = [P, C.c_longlong, P, P]
     _lib = lib
     return lib
@@ -338,6 +339,15 @@ class Engine:
 
     def lmhead_ce_fwd_bwd(self, d_loss: int | None = None):
         self._check(self.lib.ne_lmhead_ce_fwd_bwd(self._ctx, C.c_void_p(d_loss) if d_loss else None))
+
+    def lmhead_distill_fwd_bwd(self, ids: int | None = None, teacher: int | None = None, topk: int = 0,
+                               temperature: float = 1.0, hard_weight: float = 0.0,
+                               d_loss: int | None = None):
+        """lmhead_ce_fwd_bwd with a teacher's top logits (device [B*S, topk] ids and logits):
+        (1 - hard_weight) * distillation + hard_weight * cross entropy; needs head_alloc."""
+        t = TeacherDescC(ids, teacher, topk, temperature)
+        self._check(self.lib.ne_lmhead_distill_fwd_bwd(self._ctx, C.byref(t) if ids else None,
+                                                       hard_weight, d_loss))
 
     def ffn_bwd(self, layer: int):
         self._check(self.lib.ne_ffn_bwd(self._ctx, int(layer)))

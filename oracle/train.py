@@ -29,16 +29,11 @@ def _torch():
     return torch
 
 
-def forward_loss(cfg: ModelCfg, params: dict, tokens: np.ndarray, compact=None):
-    """params: torch float64 tensors {layers: [dict], rms_final, embed, qk: [(qn, kn)] or None}.
-    compact: optional compact -> full vocabulary ids; the classifier then uses
-    those embedding rows only and targets map to their compact index
-    (vocab_map_build / vocab_compact_embed, cpu_ops.h:385-422)."""
+def forward_hidden(cfg: ModelCfg, params: dict, inp):
+    """Hidden states after the final norm, [B, S, dim], of inputs [B, S];
+    params: torch float64 tensors {layers: [dict], rms_final, embed, qk: [(qn, kn)] or None}."""
     torch = _torch()
-    tok = torch.as_tensor(np.asarray(tokens, np.int64))
-    B, S1 = tok.shape
-    S = S1 - 1
-    inp, tgt = tok[:, :S], tok[:, 1:]
+    B, S = inp.shape
     hd, H, Hkv = cfg.head_dim, cfg.heads, cfg.kv_heads
     grp = H // Hkv
 
@@ -83,7 +78,18 @@ def forward_loss(cfg: ModelCfg, params: dict, tokens: np.ndarray, compact=None):
         h3 = xn @ lw["W3"].T
         g = h1 * torch.sigmoid(h1) * h3
         x = x + alpha * (g @ lw["W2"].T)
-    x = rms(x, params["rms_final"], cfg.eps)
+    return rms(x, params["rms_final"], cfg.eps)
+
+
+def forward_loss(cfg: ModelCfg, params: dict, tokens: np.ndarray, compact=None):
+    """params as forward_hidden's.
+    compact: optional compact -> full vocabulary ids; the classifier then uses
+    those embedding rows only and targets map to their compact index
+    (vocab_map_build / vocab_compact_embed, cpu_ops.h:385-422)."""
+    torch = _torch()
+    tok = torch.as_tensor(np.asarray(tokens, np.int64))
+    inp, tgt = tok[:, :-1], tok[:, 1:]
+    x = forward_hidden(cfg, params, inp)
     if compact is not None:
         c2f = torch.as_tensor(np.asarray(compact, np.int64))
         f2c = torch.full((params["embed"].shape[0],), -1, dtype=torch.int64)
@@ -98,16 +104,30 @@ def forward_loss(cfg: ModelCfg, params: dict, tokens: np.ndarray, compact=None):
     return nll.mean()
 
 
+def distill_loss(cfg: ModelCfg, params: dict, tokens: np.ndarray, ids, teacher, temperature, hard):
+    """(1 - hard) * T^2 KL(teacher's entries || model) + hard * cross entropy, mean
+    over the B*S targets; ids, teacher [B*S, K] (absent where the id is negative)."""
+    torch = _torch()
+    from . import head_loss as oh
+    tok = torch.as_tensor(np.asarray(tokens, np.int64))
+    z = (forward_hidden(cfg, params, tok[:, :-1]) @ params["embed"].T).reshape(-1, cfg.vocab)
+    keep, p, plogp = oh.distill_target(ids, teacher, cfg.vocab, temperature)
+    soft = temperature ** 2 * (plogp - (p * torch.log_softmax(z / temperature, -1)).sum(-1)) * keep
+    nll = -torch.log_softmax(z, -1).gather(-1, tok[:, 1:].reshape(-1, 1))[:, 0]
+    return ((1 - hard) * soft + hard * nll).mean()
+
+
 def loss_and_grads(cfg: ModelCfg, layers, rms_final, embed, qk, tokens, dtype="float64",
-                   compact=None):
-    """Returns (loss, grads) with grads shaped like the inputs (numpy, `dtype`)."""
+                   compact=None, loss_fn=None):
+    """Returns (loss, grads) with grads shaped like the inputs (numpy, `dtype`).
+    loss_fn(cfg, params, tokens): another loss than the cross entropy."""
     torch = _torch()
     tdt = getattr(torch, dtype)
     t = lambda a: torch.tensor(np.asarray(a), dtype=tdt, requires_grad=True)
     P = {"layers": [{k: t(v) for k, v in lw.items()} for lw in layers],
          "rms_final": t(rms_final), "embed": t(embed),
          "qk": [(t(a), t(b)) for a, b in qk] if qk is not None else None}
-    loss = forward_loss(cfg, P, tokens, compact)
+    loss = loss_fn(cfg, P, tokens) if loss_fn else forward_loss(cfg, P, tokens, compact)
     loss.backward()
     g = {"layers": [{k: v.grad.numpy() for k, v in lw.items()} for lw in P["layers"]],
          "rms_final": P["rms_final"].grad.numpy(), "embed": P["embed"].grad.numpy(),

@@ -94,3 +94,4 @@ def test_null_context_is_refused_before_anything_else():
     assert lib.ne_head_ce_bwd(None, None, None, None, None, None) == 1
     assert lib.ne_head_distill_fwd(None, None, None, None, None) == 1
     assert lib.ne_head_distill_bwd(None, None, None, None, None, None) == 1
+    assert lib.ne_lmhead_distill_fwd_bwd(None, None, 0.0, None) == 8
