@@ -25,6 +25,7 @@
 namespace ne {
 
 constexpr int HF_MAX_STAGES = 12;
+constexpr int HF_HINT_KB = 16;
 constexpr int HF_LONG_KB = 24;   // k-blocks of 64 between two takings (LONG)
 constexpr int HF_LONG_FROM = 32;
 
@@ -41,6 +42,13 @@ struct HeadLse {
   int a_rows, stages;    // rows of a box of x; ring depth
   int one_row_tile;      // all units have the same rows: one pair per CTA
 };
+
+__device__ __forceinline__ void tma_hint_2d(const void* tmap, int32_t c0, int32_t c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
 
 // A row's running statistics: sum of 2^(c2 v - mx) over the columns seen.
 struct LseRow {
@@ -132,6 +140,13 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
     }
   }
   pdl_trigger();
+  if (p.one_row_tile && warp == 2 + GEMM_EPI_WARPS && cluster < p.n_tiles) {
+    // while the kernel before this one ends: the first tile of w toward L2 (a
+    // hint; the loads that count come after the wait): about 1 us of the 15 that
+    // one token of 32000 ids, dim 768, takes.
+    const int kbs = min(p.dim_kb, HF_HINT_KB), row = cluster * p.bn + (int)crank * (p.bn / CG);
+    for (int k = lane; k < kbs; k += 32) tma_hint_2d(&w_k, k * GEMM_BK, row);
+  }
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR) cluster_sync_all();
