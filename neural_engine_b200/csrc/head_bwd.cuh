@@ -250,6 +250,9 @@ __device__ __forceinline__ void head_unit(const HeadWalk& s, const HeadOrder& o,
 __device__ __forceinline__ void flag_add(int* f) {
   asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(f) : "memory");
 }
+__device__ __forceinline__ void flag_add_relaxed(int* f) {
+  asm volatile("red.relaxed.gpu.global.add.s32 [%0], 1;" ::"l"(f) : "memory");
+}
 __device__ __forceinline__ bool flag_reached(const int* f, int want) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
@@ -684,9 +687,12 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       const bool rows_in = y0 < (w.kind == HK_DW ? ids : M);
       // dz in whole k-blocks of 64 ids: dx's product reads them
       const int cols_end = w.kind == HK_DZ ? (ids + 63) & ~63 : sp.dim;
-      // dz has been read, as far as this unit is concerned
-      if (w.kind != HK_DZ && warp == 2 && lane == 0 && crank == 0)
-        flag_add(head_flag(sp, w.piece, HF_READ));
+      // dz has been read, as far as this unit is concerned: its loads arrived
+      // before its products, and nothing this thread wrote has to be ordered (a
+      // release here waits 1,500 to 3,000 cycles for the boxes before).  With no
+      // more pieces than buffers nobody asks.
+      if (w.kind != HK_DZ && sp.pieces > HB_BUFS && warp == 2 && lane == 0 && crank == 0)
+        flag_add_relaxed(head_flag(sp, w.piece, HF_READ));
       const CUtensorMap* out = w.kind == HK_DZ ? &maps.dz_out
                                : w.kind == HK_DW ? &maps.dw_out : &maps.dx_out;
       // a warp owns half of the tile's columns and sends boxes of 128-byte rows:
