@@ -310,6 +310,23 @@ __device__ __forceinline__ void read_unit(uint32_t addr, HeadUnit& w) {
                : "memory");
 }
 
+// The producer and MMA warps run whole, on values that are the same in every
+// lane, and elect a lane for what is issued once: such values live in the
+// uniform registers that these instructions take.  Issued from a lane of its
+// own branch a k-block costs the MMA warp about 590 cycles, so 360 (its MMAs
+// take 512).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x != 0;
+}
+__device__ __forceinline__ int uniform_warp() {
+  return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort));
+}
+
 // 32 values to bf16, the low 16 bits of each word first.
 __device__ __forceinline__ void pack_bf16(const float (&v)[32], uint32_t* o) {
 #pragma unroll
@@ -383,7 +400,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gbase + (misc - base));
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + (misc - base) + 4);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform_warp();
   const int lane = threadIdx.x & 31;
   const uint32_t crank = PAIR ? cluster_ctarank() : 0u;
 
@@ -434,11 +451,13 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
   // a role other than the leader's producer takes the unit of slot `it`
   auto take = [&](int it, HeadUnit& w) -> bool {
     const int s = it % HB_SLOTS;
-    if (!mbar_wait(sfull_bar + 8 * s, (it / HB_SLOTS) & 1, sp.status, abort_flag)) return false;
+    if (!warp_wait(sfull_bar + 8 * s, (it / HB_SLOTS) & 1, sp.status, abort_flag)) return false;
     read_unit(slots + 32 * s, w);
     return true;
   };
   auto taken = [&](int it) {
+    __syncwarp();
+    if (!elect_one()) return;
     const uint32_t b = sempty_bar + 8 * (it % HB_SLOTS);
     if constexpr (PAIR) mbar_arrive_peer(mapa_shared(b, 0));
     else mbar_arrive(b);
@@ -446,7 +465,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
 
   if (warp == 0 || warp == 2 + GEMM_EPI_WARPS) {
     // ------------------------------------------------ TMA producers
-    if (lane == 0) {
+    {
       const bool is_a = warp == 0;
       const bool leads = is_a && (!PAIR || crank == 0);   // draws the units, arms the barriers
       const uint64_t pol = policy_evict_normal();
@@ -460,17 +479,17 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       uint32_t phase = 0;
       bool ok = true;
       HeadUnit nw{};   // the leader's next unit
-      // hands over the leader's next unit once what it depends on is done: dz,
-      // its buffer was read for the last time; dx and dw, dz was written, and dx
-      // was added to by the piece before.  now: wait for that.
       // What is known to be done: pieces read and added up to here, and the split
       // written last asked for (units come in the order of pieces and kinds).
       int read_to = -1, added_to = -1, made_piece = -1, made_split = -1;
       auto reached = [&](int* f, int want, bool now) -> bool {
-        if (flag_reached(f, want)) return true;
-        if (now && !flag_wait(f, want, sp.status, abort_flag)) ok = false;
+        if (__all_sync(0xffffffffu, flag_reached(f, want))) return true;
+        if (now && !__all_sync(0xffffffffu, flag_wait(f, want, sp.status, abort_flag))) ok = false;
         return now && ok;
       };
+      // hands over the leader's next unit once what it depends on is done: dz,
+      // its buffer was read for the last time; dx and dw, dz was written, and dx
+      // was added to by the piece before.  now: wait for that.
       auto hand_over = [&](int it, bool now) -> bool {
         if (nw.kind == HK_DZ) {
           const int p = nw.piece - HB_BUFS;
@@ -497,21 +516,23 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         }
         const int s = it % HB_SLOTS;
         const uint32_t at = slots + 32 * s;
-        if (!mbar_wait(sempty_bar + 8 * s, ((it / HB_SLOTS) & 1) ^ 1, sp.status, abort_flag)) {
+        if (!warp_wait(sempty_bar + 8 * s, ((it / HB_SLOTS) & 1) ^ 1, sp.status, abort_flag)) {
           ok = false;
           return false;
         }
-        st_shared_v4(at, nw.kind, nw.piece, nw.mt, nw.nt);
-        st_shared_v4(at + 16, nw.split, nw.kb0, nw.kb, nw.n);
-        mbar_arrive(sfull_bar + 8 * s);
-        if constexpr (PAIR) post_unit(mapa_shared(at, 1), mapa_shared(sfull_bar + 8 * s, 1), nw);
+        if (elect_one()) {
+          st_shared_v4(at, nw.kind, nw.piece, nw.mt, nw.nt);
+          st_shared_v4(at + 16, nw.split, nw.kb0, nw.kb, nw.n);
+          mbar_arrive(sfull_bar + 8 * s);
+          if constexpr (PAIR) post_unit(mapa_shared(at, 1), mapa_shared(sfull_bar + 8 * s, 1), nw);
+        }
         return true;
       };
       // draws the unit after the one drawn before; the latency of the counter
       // passes behind a unit's loads
       auto next_unit = [&] {
-        head_unit(sp, ord, drawn, nw);
-        if (nw.kind != HK_END) drawn = atomicAdd(sp.counters, 1);
+        head_unit(sp, ord, __shfl_sync(0xffffffffu, drawn, 0), nw);
+        if (nw.kind != HK_END && lane == 0) drawn = atomicAdd(sp.counters, 1);
       };
       if (leads) {
         next_unit();
@@ -543,19 +564,21 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         for (int k = 0; k < w.kb; ++k, k0 += GEMM_BK) {
           const uint32_t bar = full_to + 8 * stage;
           const uint32_t dst = tiles + stage * C::STAGE_BYTES + (is_a ? 0 : C::A_BYTES);
-          if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, sp.status, abort_flag)) {
+          if (!warp_wait(empty_bar + 8 * stage, phase ^ 1u, sp.status, abort_flag)) {
             ok = false;
             break;
           }
-          if (leads) mbar_arrive_expect_tx(full_bar + 8 * stage, CG * C::STAGE_BYTES);
-          if (!mn) {
-            ld(dst, tm, bar, k0, first);
-          } else {
-            ld(dst, tm, bar, first, k0);
-            ld(dst + MN_BOX, tm, bar, first + 64, k0);
-            if (!PAIR && !is_a) {   // 256 rows of B in one CTA
-              ld(dst + 2 * MN_BOX, tm, bar, first + 128, k0);
-              ld(dst + 3 * MN_BOX, tm, bar, first + 192, k0);
+          if (elect_one()) {
+            if (leads) mbar_arrive_expect_tx(full_bar + 8 * stage, CG * C::STAGE_BYTES);
+            if (!mn) {
+              ld(dst, tm, bar, k0, first);
+            } else {
+              ld(dst, tm, bar, first, k0);
+              ld(dst + MN_BOX, tm, bar, first + 64, k0);
+              if (!PAIR && !is_a) {   // 256 rows of B in one CTA
+                ld(dst + 2 * MN_BOX, tm, bar, first + 128, k0);
+                ld(dst + 3 * MN_BOX, tm, bar, first + 192, k0);
+              }
             }
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -583,7 +606,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0 && (!PAIR || crank == 0)) {
+    if (!PAIR || crank == 0) {
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -593,7 +616,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         if (!take(it, w)) break;
         taken(it);
         if (w.kind == HK_END) break;
-        if (!mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, sp.status, abort_flag)) break;
+        if (!warp_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, sp.status, abort_flag)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * HB_BN;
         const int a_mn = w.kind == HK_DW, b_mn = w.kind != HK_DZ;
@@ -602,29 +625,35 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
         bool ok = true;
         for (int k = 0; k < w.kb; ++k) {
-          if (!mbar_wait(full_bar + 8 * stage, phase, sp.status, abort_flag)) { ok = false; break; }
+          if (!warp_wait(full_bar + 8 * stage, phase, sp.status, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = tiles + stage * C::STAGE_BYTES;
-          const uint64_t ad = a_mn ? smem_desc_mn_sw128(sa, MN_BOX) : smem_desc_k_sw128(sa);
-          const uint64_t bd = b_mn ? smem_desc_mn_sw128(sa + C::A_BYTES, MN_BOX)
-                                   : smem_desc_k_sw128(sa + C::A_BYTES);
+          if (elect_one()) {
+            const uint32_t sa = tiles + stage * C::STAGE_BYTES;
+            const uint64_t ad = a_mn ? smem_desc_mn_sw128(sa, MN_BOX) : smem_desc_k_sw128(sa);
+            const uint64_t bd = b_mn ? smem_desc_mn_sw128(sa + C::A_BYTES, MN_BOX)
+                                     : smem_desc_k_sw128(sa + C::A_BYTES);
 #pragma unroll
-          for (int j = 0; j < GEMM_BK / 16; ++j)
-            if constexpr (PAIR)
-              umma_f16_pair(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
-            else
-              umma_f16(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
-          if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
-          else umma_commit(empty_bar + 8 * stage);
+            for (int j = 0; j < GEMM_BK / 16; ++j)
+              if constexpr (PAIR)
+                umma_f16_pair(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
+              else
+                umma_f16(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
+            if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
+            else umma_commit(empty_bar + 8 * stage);
+          }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
-        else umma_commit(tfull_bar + 8 * acc);
+        if (elect_one()) {
+          if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
+          else umma_commit(tfull_bar + 8 * acc);
+        }
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
-      if constexpr (PAIR) umma_commit_pair(drain_bar, 0x1);
-      else umma_commit(drain_bar);
+      if (elect_one()) {
+        if constexpr (PAIR) umma_commit_pair(drain_bar, 0x1);
+        else umma_commit(drain_bar);
+      }
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(drain_bar, 0)) {
         if (globaltimer_ns() - t0 > 100000000ull) break;
@@ -653,10 +682,8 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       if (lane == 0 && owed && !mbar_try_wait(sfull_bar + 8 * (it % HB_SLOTS), (it / HB_SLOTS) & 1))
         settle();
       HeadUnit w;
-      const bool got = take(it, w);
-      if (!__all_sync(0xffffffffu, got)) break;
-      __syncwarp();
-      if (lane == 0) taken(it);
+      if (!take(it, w)) break;
+      taken(it);
       if (w.kind == HK_END) break;
       const int id0 = w.piece * sp.piece;
       const int ids = w.piece == sp.pieces - 1 ? ord.last_ids : sp.piece;
@@ -679,8 +706,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         cursor_seek<true>(dzp.t, cur, m, count, id0 + n_tile + 128 * half);
       }
       if (lane == 0 && owed && !mbar_try_wait(tfull_bar + 8 * acc, acc_phase)) settle();
-      const bool ready = mbar_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag);
-      if (!__all_sync(0xffffffffu, ready)) break;
+      if (!warp_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * HB_BN;
       const bool b16 = w.kind == HK_DZ || (w.kind == HK_DW && !sp.dw_f32);

@@ -109,7 +109,7 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(gbase + 16 * HF_MAX_STAGES + 44);
   const uint32_t b_at = base + 1024, a_at = b_at + stages * b_bytes;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform_warp();
   const int lane = threadIdx.x & 31;
   const uint32_t crank = PAIR ? cluster_ctarank() : 0u;
   const int cluster = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
@@ -162,50 +162,50 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
 
   if (warp == 0 || warp == 2 + GEMM_EPI_WARPS) {
     // ------------------------------------------------ TMA producers
-    if (lane == 0) {
-      const bool is_a = warp == 0;
-      const bool arms = is_a && (!PAIR || crank == 0);
-      // x is read again for every tile of ids, w once for all tiles of rows
-      const uint64_t pol = is_a ? policy_evict_last() : policy_evict_normal();
-      const uint32_t full_to = PAIR ? mapa_shared(full_bar, 0) : full_bar;
-      const CUtensorMap* tm = is_a ? &x_k : &w_k;
-      const uint32_t ring = is_a ? a_at : b_at, bytes = is_a ? a_bytes : b_bytes;
-      const uint32_t expect = CG * (a_bytes + b_bytes);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int u = cluster; u < units && ok; u += clusters) {
-        int mt, nt, sp_unused;
-        unit_coords(sh, u, mt, nt, sp_unused);
-        const int first = is_a ? mt * TILE_M + (int)crank * GEMM_BM
-                               : nt * p.bn + (int)crank * (p.bn / CG);
-        for (int k = 0; k < p.dim_kb; ++k) {
-          if (!mbar_wait(empty_bar + 8 * stage, phase ^ 1u, p.status, abort_flag)) {
-            ok = false;
-            break;
-          }
+    const bool is_a = warp == 0;
+    const bool arms = is_a && (!PAIR || crank == 0);
+    // x is read again for every tile of ids, w once for all tiles of rows
+    const uint64_t pol = is_a ? policy_evict_last() : policy_evict_normal();
+    const uint32_t full_to = PAIR ? mapa_shared(full_bar, 0) : full_bar;
+    const CUtensorMap* tm = is_a ? &x_k : &w_k;
+    const uint32_t ring = is_a ? a_at : b_at, bytes = is_a ? a_bytes : b_bytes;
+    const uint32_t expect = CG * (a_bytes + b_bytes);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int u = cluster; u < units && ok; u += clusters) {
+      int mt, nt, sp_unused;
+      unit_coords(sh, u, mt, nt, sp_unused);
+      const int first = is_a ? mt * TILE_M + (int)crank * GEMM_BM
+                             : nt * p.bn + (int)crank * (p.bn / CG);
+      for (int k = 0; k < p.dim_kb; ++k) {
+        if (!warp_wait(empty_bar + 8 * stage, phase ^ 1u, p.status, abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
           if (arms) mbar_arrive_expect_tx(full_bar + 8 * stage, expect);
           if constexpr (PAIR)
             tma_load_2d_pair(ring + stage * bytes, tm, full_to + 8 * stage, k * GEMM_BK, first, pol);
           else
             tma_load_2d(ring + stage * bytes, tm, full_to + 8 * stage, k * GEMM_BK, first, pol);
-          if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
+        if (++stage == stages) { stage = 0; phase ^= 1u; }
       }
-      // no load may be in flight when the CTA exits (gemm_tc.cuh)
-      if (arms) {
-        for (int s = 0; s < stages; ++s) {
-          const uint32_t par = (s < stage) ? phase : (phase ^ 1u);
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(full_bar + 8 * s, par)) {
-            if (globaltimer_ns() - t0 > 100000000ull) break;
-          }
+    }
+    // no load may be in flight when the CTA exits (gemm_tc.cuh)
+    if (arms) {
+      for (int s = 0; s < stages; ++s) {
+        const uint32_t par = (s < stage) ? phase : (phase ^ 1u);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(full_bar + 8 * s, par)) {
+          if (globaltimer_ns() - t0 > 100000000ull) break;
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0 && (!PAIR || crank == 0)) {
+    if (!PAIR || crank == 0) {
       const uint32_t idesc = umma_idesc_f16(TILE_M, p.bn, 1);
       int stage = 0;
       uint32_t phase = 0;
@@ -214,31 +214,37 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
       bool ok = true;
       for (int u = cluster; u < units && ok; u += clusters) {
         for (int k0 = 0; k0 < p.dim_kb && ok; k0 += LONG ? HF_LONG_KB : p.dim_kb) {
-          if (!mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, p.status, abort_flag)) { ok = false; break; }
+          if (!warp_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, p.status, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * HB_BN;
           const int kn = LONG ? min(HF_LONG_KB, p.dim_kb - k0) : p.dim_kb;
           for (int k = 0; k < kn; ++k) {
-            if (!mbar_wait(full_bar + 8 * stage, phase, p.status, abort_flag)) { ok = false; break; }
+            if (!warp_wait(full_bar + 8 * stage, phase, p.status, abort_flag)) { ok = false; break; }
             tc_fence_after();
-            const uint64_t ad = smem_desc_k_sw128(a_at + stage * a_bytes);
-            const uint64_t bd = smem_desc_k_sw128(b_at + stage * b_bytes);
+            if (elect_one()) {
+              const uint64_t ad = smem_desc_k_sw128(a_at + stage * a_bytes);
+              const uint64_t bd = smem_desc_k_sw128(b_at + stage * b_bytes);
 #pragma unroll
-            for (int j = 0; j < GEMM_BK / 16; ++j)
-              if constexpr (PAIR) umma_f16_pair(d_tmem, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0);
-              else umma_f16(d_tmem, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0);
-            if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
-            else umma_commit(empty_bar + 8 * stage);
+              for (int j = 0; j < GEMM_BK / 16; ++j)
+                if constexpr (PAIR) umma_f16_pair(d_tmem, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0);
+                else umma_f16(d_tmem, ad + 2 * j, bd + 2 * j, idesc, (k | j) != 0);
+              if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
+              else umma_commit(empty_bar + 8 * stage);
+            }
             if (++stage == stages) { stage = 0; phase ^= 1u; }
           }
           if (!ok) break;
-          if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
-          else umma_commit(tfull_bar + 8 * acc);
+          if (elect_one()) {
+            if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
+            else umma_commit(tfull_bar + 8 * acc);
+          }
           if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
       }
-      if constexpr (PAIR) umma_commit_pair(drain_bar, 0x1);
-      else umma_commit(drain_bar);
+      if (elect_one()) {
+        if constexpr (PAIR) umma_commit_pair(drain_bar, 0x1);
+        else umma_commit(drain_bar);
+      }
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(drain_bar, 0)) {
         if (globaltimer_ns() - t0 > 100000000ull) break;
