@@ -399,9 +399,11 @@ NE_API ne_status ne_sdpa_fwd_device(ne_ctx* ctx, const void* d_q, const void* d_
  * All calls only enqueue work on the context's stream, use the workspaces of
  * ne_head_alloc and may be captured into a graph.  dim, ldx, ldw, lddx and
  * lddw are multiples of 8, x, w, dx and dw 16-byte aligned; rows, vocab and
- * topk are arbitrary (rows may be 0).  Outputs are the same bits every time.
- * A target or id >= vocab counts as absent and is reported by the next call
- * that synchronises (NE_ERR_BOUNDS). */
+ * topk are arbitrary (rows may be 0).  Outputs must not overlap inputs, and are
+ * the same bits every time.  The workspaces belong to one call at a time: graphs
+ * of these calls are replayed one after the other.  A target or id >= vocab
+ * counts as absent and is reported by the next call that synchronises
+ * (NE_ERR_BOUNDS). */
 typedef struct ne_head_desc {
   const void* x; long long ldx;   /* bf16 [rows, dim]: hidden states after the final norm */
   const void* w; long long ldw;   /* bf16 [vocab, dim] */

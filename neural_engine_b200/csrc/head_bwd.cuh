@@ -13,10 +13,10 @@
 // enough to be read back from L2.  The leading CTA's A producer draws units from
 // a counter in device memory, waits until the units it depends on have
 // signalled, and hands it to the other roles of both CTAs through a ring of
-// slots.  A unit depends only on units drawn
-// before it, so the wait ends whatever the number of CTAs that run; it is
-// bounded all the same.  Which pair computes a unit changes no value: every
-// unit is computed whole, and dx adds the pieces in their order.
+// slots.  A unit depends only on units drawn before it, so the wait ends
+// whatever the number of CTAs that run; it is bounded all the same.  Which pair
+// computes a unit changes no value: every unit is computed whole, and dx adds
+// the pieces in their order.
 // As launches of their own the products left 14% of the pairs idle in their last
 // waves (4096 rows, dim 1024: 64 tiles of dx, 128 of dw, for 74 pairs).
 //
@@ -313,8 +313,8 @@ __device__ __forceinline__ void read_unit(uint32_t addr, HeadUnit& w) {
 // The producer and MMA warps run whole, on values that are the same in every
 // lane, and elect a lane for what is issued once: such values live in the
 // uniform registers that these instructions take.  Issued from a lane of its
-// own branch a k-block costs the MMA warp about 590 cycles, so 360 (its MMAs
-// take 512).
+// own branch a k-block costs the MMA warp about 590 cycles, this way 360 (the
+// MMAs take 512).
 __device__ __forceinline__ bool elect_one() {
   uint32_t x;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(x));

@@ -13,14 +13,13 @@
 // minus a sparse target.  So both run on
 //   pack      rows that count, moved together (masked rows cost no product and
 //             what stands in them, NaN included, reaches nothing)
-//   teacher   p and the ids of each row, sorted and without repeats (distillation)
+//   teacher   p and the ids of each row, sorted (distillation)
 //   forward   x . w^T on the tensor cores; the epilogue keeps per row a running
 //             maximum and sum of exp2 and picks out the target's logits
 //   join      the tiles' (maximum, sum) pairs of a row -> lse, loss
 //   backward  per piece of the vocabulary: the logits again, turned into bf16 dz
 //             by the epilogue, then dx += dz . w and dw = dz^T . x
-// Everything is ordered by the stream and by tiles: no atomics, the same bits
-// every time.
+// Nothing is added up in an order that could change: the same bits every time.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -70,9 +69,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kTopkMax = 256;
 // dz of one piece (three are alive), and the slabs dx is summed in where its
-// product is split.  4096 rows of 151936 ids, dim 1024, backward pass: 3.41 ms with
-// pieces of 32 MB, 3.26 with 64, 3.18 with 128, 3.11 with 256 (1.2 GB would be
-// all of dz): longer sums per unit of dx against room.
+// product is split.  Backward pass of 4096 rows with pieces of 32, 64, 128 and 256
+// MB: 3.14, 3.15, 3.15, 3.10 ms (151936 ids, dim 1024; all of dz would be 1.2 GB),
+// 0.262, 0.261, 0.245, 0.240 (32000 ids, dim 768, six rows in ten left out).
 constexpr size_t kPieceBytes = 128u << 20;
 constexpr size_t kSlabBytes = 64u << 20;
 
@@ -85,16 +84,19 @@ __device__ __forceinline__ bool row_counts(const int32_t* target, const int* kee
   return t >= 0 && t < vocab;
 }
 
-// Moves the rows that count together, in order.  A block takes 8 to 32 rows; how
-// many count before them it counts itself (the targets stay in L2: 4 bytes a
-// row, once per block), so there is no scan to wait for.
+// Moves the rows that count together, in order.  A block takes up to 32 rows at a
+// time; how many count before its first one it counts itself (the targets stay
+// in L2: 4 bytes a row, once per block), so there is no scan to wait for.  With
+// more than 8192 rows a block takes several such groups, which bounds the blocks
+// and so the counting.
 constexpr int PACK_ROWS = 32;
 int pack_rows(int rows) { return rows <= 2048 ? 8 : rows <= 8192 ? 16 : PACK_ROWS; }
+int pack_groups(int rows) { return (rows + 8191) / 8192; }
 struct HeadPack {
   const __nv_bfloat16* x;
   long long ldx;
   int rows, dim, vocab;
-  int per;                  // rows a block
+  int per, groups;          // rows a group, groups a block
   const int32_t* target;    // cross entropy
   const int* keep;          // distillation
   int* row_of;
@@ -122,49 +124,56 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
   const int rows = p.rows, vocab = p.vocab, per = p.per;
   __shared__ int before, base_s;
   __shared__ unsigned mask_s;
-  const int first = blockIdx.x * per;
+  const int block_first = blockIdx.x * per * p.groups;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) before = 0;
   __syncthreads();
   int n = 0;
-  for (int i = threadIdx.x; i < first; i += 256) n += row_counts(target, keep, i, vocab);
+  for (int i = threadIdx.x; i < block_first; i += 256) n += row_counts(target, keep, i, vocab);
   n = __reduce_add_sync(0xffffffffu, n);
   if (lane == 0 && n) atomicAdd(&before, n);
   __syncthreads();
-  if (warp == 0) {
-    const int i = first + lane;
-    const bool mine = lane < per && i < rows;
-    const bool on = mine && row_counts(target, keep, i, vocab);
-    if (!keep && mine && target[i] >= vocab) atomicExch(p.status, DEV_ERR_BOUNDS);
-    const unsigned mask = __ballot_sync(0xffffffffu, on);
-    const int pos = before + __popc(mask & ((1u << lane) - 1));
-    if (mine) p.pos_of[i] = on ? pos : -1;
-    if (on) {
-      p.row_of[pos] = i;
-      if (target) p.target_p[pos] = target[i];
-      if (p.coef) {
-        const float a = (p.grad ? p.grad[i] : 1.0f) * p.factor;
-        p.coef[pos] = make_float2(a, log2f(fabsf(a)) - p.lse[i] * kLog2e);
+  for (int g = 0; g < p.groups; ++g) {
+    const int first = block_first + g * per;
+    if (first >= rows) break;
+    if (warp == 0) {
+      const int i = first + lane, base = before;
+      const bool mine = lane < per && i < rows;
+      const bool on = mine && row_counts(target, keep, i, vocab);
+      if (!keep && mine && target[i] >= vocab) atomicExch(p.status, DEV_ERR_BOUNDS);
+      const unsigned mask = __ballot_sync(0xffffffffu, on);
+      const int pos = base + __popc(mask & ((1u << lane) - 1));
+      if (mine) p.pos_of[i] = on ? pos : -1;
+      if (on) {
+        p.row_of[pos] = i;
+        if (target) p.target_p[pos] = target[i];
+        if (p.coef) {
+          const float a = (p.grad ? p.grad[i] : 1.0f) * p.factor;
+          p.coef[pos] = make_float2(a, log2f(fabsf(a)) - p.lse[i] * kLog2e);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mask_s = mask;
+        base_s = base;
+        before = base + __popc(mask);
       }
     }
-    if (lane == 0) {
-      mask_s = mask;
-      base_s = before;
-    }
-  }
-  __syncthreads();
-  const unsigned mask = mask_s;
-  const int vecs = p.dim / 8;
-  for (int r = warp; r < per; r += 8) {
-    if (!((mask >> r) & 1u)) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(p.x + (long long)(first + r) * p.ldx);
-    uint4* dst = reinterpret_cast<uint4*>(
-        p.xp + (long long)(base_s + __popc(mask & ((1u << r) - 1))) * p.ldp);
+    __syncthreads();
+    const unsigned mask = mask_s;
+    const int base = base_s, vecs = p.dim / 8;
+    for (int r = warp; r < per; r += 8) {
+      if (!((mask >> r) & 1u)) continue;
+      const uint4* src = reinterpret_cast<const uint4*>(p.x + (long long)(first + r) * p.ldx);
+      uint4* dst = reinterpret_cast<uint4*>(
+          p.xp + (long long)(base + __popc(mask & ((1u << r) - 1))) * p.ldp);
 #pragma unroll 4
-    for (int k = lane; k < vecs; k += 32) dst[k] = src[k];
+      for (int k = lane; k < vecs; k += 32) dst[k] = src[k];
+    }
+    __syncthreads();   // mask_s and base_s are free again
   }
   if (blockIdx.x == gridDim.x - 1) {
-    const int total = base_s + __popc(mask);
+    const int total = before;
     const int stop = total > 64 ? (total + 63) / 64 * 64 : 64;
     if (threadIdx.x == 0) *p.count = total;
     // zero rows up to a whole block of 64, which dw's product reduces over
@@ -444,7 +453,7 @@ ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
                 std::string(what) + ": ldx and ldw must be multiples of 8, at least dim");
   if ((reinterpret_cast<uintptr_t>(d->x) | reinterpret_cast<uintptr_t>(d->w)) & 15u)
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x and w must be 16-byte aligned");
-  if (!(d->scale > 0.f) || !std::isfinite(d->scale))
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale * kLog2e))
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": scale must be positive and finite");
   const HeadState* h = ctx->head;
   if (!h || d->rows > h->max_rows || d->dim > h->max_dim || d->vocab > h->max_vocab)
@@ -452,13 +461,16 @@ ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
   return NE_OK;
 }
 
-ne_status teacher_check(ne_ctx* ctx, const ne_teacher_desc* t, const char* what) {
+ne_status teacher_check(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t, const char* what) {
   if (!t->ids || !t->logits || t->topk <= 0)
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": teacher ids, logits or topk missing");
   if (t->topk > kTopkMax)
     return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": topk is at most 256");
   if (!(t->temperature > 0.f) || !std::isfinite(t->temperature))
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature must be positive and finite");
+  if (!std::isfinite(t->temperature * t->temperature) ||
+      !std::isfinite(d->scale / t->temperature * kLog2e) || !std::isfinite(1.0f / t->temperature))
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature out of range");
   if (t->topk > ctx->head->max_topk)
     return fail(ctx, NE_ERR_STATE, std::string(what) + ": ne_head_alloc has no room for this topk");
   return NE_OK;
@@ -470,8 +482,8 @@ ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
   if (!c.teacher) return NE_OK;
   HeadState* h = ctx->head;
   const int rows = c.d->rows;
-  NE_LAUNCH(launch_k(head_teacher_kernel, dim3(rows), dim3((unsigned)up(c.n, 32)), 0, ctx->st, c.teacher->ids, c.teacher->logits, rows,
-                     c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->tab, tab_entries(c.d->vocab),
+  NE_LAUNCH(launch_k(head_teacher_kernel, dim3(rows), dim3((unsigned)up(c.n, 32)), 0, ctx->st,
+                     c.teacher->ids, c.teacher->logits, rows, c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->tab, tab_entries(c.d->vocab),
                      h->neg_entropy, h->keep, ctx->d_status));
   return NE_OK;
 }
@@ -486,6 +498,8 @@ ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, const float* lse, const f
   p.dim = c.d->dim;
   p.vocab = c.d->vocab;
   p.per = pack_rows(p.rows);
+  p.groups = pack_groups(p.rows);
+  const int block_rows = p.per * p.groups;
   p.target = c.target;
   p.keep = c.teacher ? h->keep : nullptr;
   p.row_of = h->row_of;
@@ -501,7 +515,8 @@ ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, const float* lse, const f
   p.counters = h->counters;
   p.n_counters = counters;
   p.status = ctx->d_status;
-  NE_LAUNCH(launch_k(head_pack_kernel, dim3((p.rows + p.per - 1) / p.per), dim3(256), 0, ctx->st, p));
+  NE_LAUNCH(launch_k(head_pack_kernel, dim3((p.rows + block_rows - 1) / block_rows),
+                     dim3(256), 0, ctx->st, p));
   return NE_OK;
 }
 
@@ -562,7 +577,8 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   p.stages = plan.stages;
   p.one_row_tile = plan.one_row_tile;
   CUtensorMap x, w;
-  if (!make_tmap(&x, plan.packed ? h->xp : d.x, rows, D, plan.packed ? (long long)up(D, GEMM_BK) : d.ldx, plan.a_rows, 0) ||
+  const long long ldx = plan.packed ? (long long)up(D, GEMM_BK) : d.ldx;
+  if (!make_tmap(&x, plan.packed ? h->xp : d.x, rows, D, ldx, plan.a_rows, 0) ||
       !make_tmap(&w, d.w, V, D, d.ldw, plan.bn / plan.cg, 0))
     return fail(ctx, NE_ERR_CUDA, "head loss: tensor map");
   const bool lng = p.dim_kb > HF_LONG_FROM;   // long sums (head_fwd.cuh)
@@ -744,7 +760,7 @@ ne_status head_train(ne_ctx* ctx, const ne_head_desc* d, const int32_t* target,
                      float* dw) {
   const char* what = "ne_lmhead_distill_fwd_bwd";
   ne_status s = head_check(ctx, d, what);
-  if (s != NE_OK || (teacher && (s = teacher_check(ctx, teacher, what)) != NE_OK)) return s;
+  if (s != NE_OK || (teacher && (s = teacher_check(ctx, d, teacher, what)) != NE_OK)) return s;
   const ne_head_grads g{dx, d->dim, 1, dw, d->dim, 1};
   HeadCall c;
   c.d = d;
@@ -887,7 +903,7 @@ NE_API ne_status ne_head_distill_fwd(ne_ctx* ctx, const ne_head_desc* d, const n
   if (!d_loss || !d_lse)
     return fail(ctx, NE_ERR_INVALID, "ne_head_distill_fwd: loss or lse is NULL");
   ne_status s = head_check(ctx, d, "ne_head_distill_fwd");
-  if (s != NE_OK || (s = teacher_check(ctx, t, "ne_head_distill_fwd")) != NE_OK || d->rows == 0)
+  if (s != NE_OK || (s = teacher_check(ctx, d, t, "ne_head_distill_fwd")) != NE_OK || d->rows == 0)
     return s;
   NE_CUDA(cudaSetDevice(ctx->device));
   HeadCall c;
@@ -904,7 +920,7 @@ NE_API ne_status ne_head_distill_bwd(ne_ctx* ctx, const ne_head_desc* d, const n
   if (!ctx || !d || !t || !g) return NE_ERR_INVALID;
   if (!d_lse) return fail(ctx, NE_ERR_INVALID, "ne_head_distill_bwd: lse is NULL");
   ne_status s = head_check(ctx, d, "ne_head_distill_bwd");
-  if (s != NE_OK || (s = teacher_check(ctx, t, "ne_head_distill_bwd")) != NE_OK ||
+  if (s != NE_OK || (s = teacher_check(ctx, d, t, "ne_head_distill_bwd")) != NE_OK ||
       (s = grads_check(ctx, d, g, "ne_head_distill_bwd")) != NE_OK)
     return s;
   NE_CUDA(cudaSetDevice(ctx->device));

@@ -260,6 +260,41 @@ def test_several_pieces_of_the_vocabulary(eng):
         assert float(over.max()) <= 0
 
 
+@pytest.mark.parametrize("rows", [8192, 8193, 20011])
+def test_many_rows(eng, rows):
+    """Rows beyond 8192 are packed several groups a block."""
+    h = Head(rows, 64, 130, seed=rows).ce(0.5)
+    h.target[5000:7500] = -7          # whole groups without a row that counts
+    h.run(eng).check()
+    Head(rows, 64, 130, seed=rows).distill(3, masked=0.6).run(eng).check()
+
+
+def test_two_contexts_at_once():
+    """Two contexts' passes enqueued on their streams together: neither's units
+    wait for CTAs that the other keeps off the SMs."""
+    import neural_engine_b200 as ne
+    es = [ne.Engine(ne.ModelConfig(1, 128, 256, 2, 2, 64, 256)) for _ in range(2)]
+    hs = [Head(1500, 136, 9001, seed=21).ce(0.2), Head(700, 264, 12000, seed=22).distill(11, 2.0)]
+    for e, h in zip(es, hs):
+        h.upload()
+        e.head_alloc(h.rows, h.dim, h.vocab, h.topk)
+    for _ in range(8):
+        for e, h in zip(es, hs):
+            h.forward(e)
+            h.backward(e)
+    for e in es:
+        e.sync()
+    got = [[t.clone() for t in (h.loss, h.lse, h.dx, h.dw)] for h in hs]
+    for e, h, a in zip(es, hs, got):
+        h.upload()
+        h.forward(e)
+        h.backward(e)
+        e.sync()
+        for u, v in zip(a, (h.loss, h.lse, h.dx, h.dw)):
+            assert torch.equal(u, v)
+        e.close()
+
+
 def test_the_same_bits_every_time(eng):
     for h in (Head(700, 136, 3001, seed=9).ce(0.3), Head(700, 136, 3001, seed=9).distill(20, 2.0)):
         h.run(eng)
@@ -367,7 +402,8 @@ def test_refusals():
             refused(1, fn, base, **kw)
     for fn, base in ((eng.head_distill_fwd, kd), (eng.head_distill_bwd, kdb)):
         for kw in (dict(ids=None), dict(teacher=None), dict(topk=0), dict(topk=-3), dict(temperature=0.0),
-                   dict(temperature=NAN), dict(temperature=-1.0)):
+                   dict(temperature=NAN), dict(temperature=-1.0), dict(temperature=1e-45),
+                   dict(temperature=1e30)):
             refused(1, fn, base, **kw)
         refused(7, fn, base, topk=257)
         refused(8, fn, base, topk=256)
