@@ -442,7 +442,8 @@ NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_
                                 float* d_loss, float* d_lse);
 /* Gradients of sum_i grad_i loss_i, from the d_lse of ne_head_ce_fwd; d_grad
  * [rows] NULL: ones.  dz = grad (softmax - onehot) is rounded to bf16 as the
- * operand of the tensor-core products that give dx and dw. */
+ * operand of the tensor-core products that give dx and dw; with at most 64 rows
+ * that count it is kept in two bf16 parts. */
 NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
                                 const float* d_lse, const float* d_grad, const ne_head_grads* g);
 

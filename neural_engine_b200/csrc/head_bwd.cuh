@@ -33,6 +33,7 @@ constexpr int HB_BN = 256;
 constexpr int HB_SLOTS = 8;
 constexpr int HB_THREADS = GEMM_THREADS + 32;   // warps: A, MMA, 8 x epilogue, B
 constexpr int HB_BOX = 4096;                    // 32 rows of 128 bytes
+constexpr int HB_TWIN = 64;                     // up to here rows stand twice
 constexpr int HB_TAB = 256;                     // ids per entry of a row's index
 
 template <int CG>
@@ -130,6 +131,7 @@ struct HeadDz {
 
 struct HeadMaps {
   CUtensorMap x_k, w_k;        // dz: operands (K = dim contiguous)
+  CUtensorMap twin_k, twin_mn; // x_k, x_mn of the rows that stand twice
   CUtensorMap dz_out;          // dz: [buffers * rows64][piece]
   CUtensorMap dz_k, w_mn;      // dx: dz (K = ids), w as [ids][dim]
   CUtensorMap dx_out;          // dx: [splits * rows64][dim] fp32
@@ -439,9 +441,12 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
   pdl_wait();
   // the leader's A producer draws its first unit while the row count arrives
   int drawn = threadIdx.x == 0 && crank == 0 ? atomicAdd(sp.counters, 1) : 0;
-  // whole blocks of 64 rows, at least one (its rows are zeros)
+  // whole blocks of 64 rows; rows behind the last are zeros
   const int count = *sp.d_rows;
-  const int blocks = max((count + GEMM_BK - 1) / GEMM_BK, 1);
+  // up to 64 rows stand twice in a tile that has room for them anyway, for dz in
+  // two bf16 parts
+  const bool twin = count <= HB_TWIN;
+  const int blocks = twin ? 2 : (count + GEMM_BK - 1) / GEMM_BK;
   const int M = blocks * GEMM_BK, m_tiles = (M + TILE_M - 1) / TILE_M;
   const int last_ids = sp.vocab - (sp.pieces - 1) * sp.piece;
   const HeadCounts full = head_counts(sp, m_tiles, TILE_M, sp.piece);
@@ -553,8 +558,10 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         // this role's operand: K-major is one box, MN-major one per 64 columns
         const bool mn = is_a ? w.kind == HK_DW : w.kind != HK_DZ;
         const CUtensorMap* tm =
-            is_a ? (w.kind == HK_DZ ? &maps.x_k : w.kind == HK_DX ? &maps.dz_k : &maps.dz_mn)
-                 : (w.kind == HK_DZ ? &maps.w_k : w.kind == HK_DX ? &maps.w_mn : &maps.x_mn);
+            is_a ? (w.kind == HK_DZ ? (twin ? &maps.twin_k : &maps.x_k)
+                    : w.kind == HK_DX ? &maps.dz_k : &maps.dz_mn)
+                 : (w.kind == HK_DZ ? &maps.w_k
+                    : w.kind == HK_DX ? &maps.w_mn : twin ? &maps.twin_mn : &maps.x_mn);
         // first row (K-major) or column (MN-major) of the tile, and where K starts
         const int first = is_a ? w.mt * TILE_M + (int)crank * GEMM_BM + (w.kind == HK_DX ? buf_row : 0)
                                : w.nt * HB_BN + (int)crank * (w.n / CG) + (w.kind == HK_DZ ? id0 : 0);
@@ -695,7 +702,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       float mag = 0.f, shift = 0.f;
       uint32_t keep = 0u, sign = 0u;
       if (w.kind == HK_DZ) {
-        const int m = y0 + lane;
+        const int m = (twin ? y0 & (HB_TWIN - 1) : y0) + lane;
         if (m < count) {
           const float2 co = dzp.coef[m];
           mag = fabsf(co.x);
@@ -757,7 +764,13 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
               }
             }
             // rounded once to bf16: dz is the operand of two tensor-core
-            // products, dw the caller's type
+            // products, dw the caller's type.  Where rows stand twice, the second
+            // 64 take what the rounding of the first leaves: with few rows the
+            // error of one large dz (a target's) does not average out
+            if (w.kind == HK_DZ && twin && y0 >= HB_TWIN) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+            }
             pack_bf16(v, o + 16 * h);
           }
           if (w.kind == HK_DZ) {

@@ -57,9 +57,10 @@ struct HeadState {
   float* lse = nullptr;           // [rows] between the passes of head_train
   float2* stats = nullptr;        // (max, sum exp2) of each row and half tile
   __nv_bfloat16* xp = nullptr;    // [rows up to 256][dim up to 64] packed x
+  __nv_bfloat16* twin = nullptr;  // [128][dim up to 64] the first 64 packed rows, twice
   __nv_bfloat16* dz = nullptr;    // [3][rows up to 64][piece]
   float* dx = nullptr;            // [splits][rows up to 64][dim] sums over the pieces
-  int* counters = nullptr;        // of the backward pass: units drawn, three per piece
+  int* counters = nullptr;        // of the backward pass: units drawn, flags of the pieces
 };
 
 namespace {
@@ -110,6 +111,7 @@ struct HeadPack {
   const float* grad;        // NULL: ones
   float factor;             // T * scale (* the loss's weight)
   float2* coef;             // NULL: forward
+  __nv_bfloat16* twin;      // [128][ldp] the first 64 packed rows, twice
   int* counters;
   int n_counters;
   int* status;
@@ -165,10 +167,16 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
     for (int r = warp; r < per; r += 8) {
       if (!((mask >> r) & 1u)) continue;
       const uint4* src = reinterpret_cast<const uint4*>(p.x + (long long)(first + r) * p.ldx);
-      uint4* dst = reinterpret_cast<uint4*>(
-          p.xp + (long long)(base + __popc(mask & ((1u << r) - 1))) * p.ldp);
+      const int pos = base + __popc(mask & ((1u << r) - 1));
+      uint4* dst = reinterpret_cast<uint4*>(p.xp + (long long)pos * p.ldp);
+      uint4* two = p.coef && pos < HB_TWIN ? reinterpret_cast<uint4*>(p.twin + (long long)pos * p.ldp)
+                                           : nullptr;
 #pragma unroll 4
-      for (int k = lane; k < vecs; k += 32) dst[k] = src[k];
+      for (int k = lane; k < vecs; k += 32) {
+        const uint4 v = src[k];
+        dst[k] = v;
+        if (two) two[k] = two[k + HB_TWIN * (p.ldp / 8)] = v;
+      }
     }
     __syncthreads();   // mask_s and base_s are free again
   }
@@ -178,9 +186,14 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
     if (threadIdx.x == 0) *p.count = total;
     // zero rows up to a whole block of 64, which dw's product reduces over
     const int line = (int)(p.ldp / 8);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
     uint4* z = reinterpret_cast<uint4*>(p.xp + (long long)total * p.ldp);
-    for (long long k = threadIdx.x; k < (long long)(stop - total) * line; k += 256)
-      z[k] = make_uint4(0, 0, 0, 0);
+    for (long long k = threadIdx.x; k < (long long)(stop - total) * line; k += 256) z[k] = zero;
+    if (p.coef && total < HB_TWIN) {
+      z = reinterpret_cast<uint4*>(p.twin + (long long)total * p.ldp);
+      for (int k = threadIdx.x; k < (HB_TWIN - total) * line; k += 256)
+        z[k] = z[k + HB_TWIN * line] = zero;
+    }
   }
 }
 
@@ -352,7 +365,7 @@ template <class T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int slabs,
                                                       long long slab, int rows, int dim,
                                                       const int* __restrict__ pos_of, T* dx,
-                                                      long long ld, int add) {
+                                                      long long ld, int add, const int* count) {
   pdl_trigger();
   pdl_wait();
   const int quads = dim / 4;
@@ -362,11 +375,16 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
   const int pos = pos_of[i];
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (pos >= 0) {
+    const bool twin = *count <= HB_TWIN;
     const float4* src = reinterpret_cast<const float4*>(acc + (long long)pos * dim) + k;
 #pragma unroll 8
     for (int u = 0; u < slabs; ++u) {
       const float4 q = src[u * (slab / 4)];
       v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+      if (twin) {   // the product of dz's second part, 64 rows further
+        const float4 r = src[u * (slab / 4) + HB_TWIN * quads];
+        v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
+      }
     }
   }
   T* dst = dx + (long long)i * ld + 4 * k;
@@ -514,6 +532,7 @@ ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, const float* lse, const f
   p.coef = lse ? h->coef : nullptr;
   p.counters = h->counters;
   p.n_counters = counters;
+  p.twin = h->twin;
   p.status = ctx->d_status;
   NE_LAUNCH(launch_k(head_pack_kernel, dim3((p.rows + block_rows - 1) / block_rows),
                      dim3(256), 0, ctx->st, p));
@@ -670,8 +689,8 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   HeadState* h = ctx->head;
   const ne_head_desc& d = *c.d;
   const int rows = d.rows, V = d.vocab, D = d.dim;
-  const int rows64 = (int)up(rows, 64);
-  const HeadPlan plan = head_plan(rows, D, V, ctx->num_sms);
+  const int rows64 = std::max((int)up(rows, 64), 2 * HB_TWIN);   // few rows stand twice
+  const HeadPlan plan = head_plan(rows64, D, V, ctx->num_sms);
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK ||
       (s = enqueue_pack(ctx, c, lse, grad, 1 + plan.pieces * (2 + plan.splits))) != NE_OK)
@@ -692,7 +711,9 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
             make_tmap_out(&maps.dx_out, h->dx, plan.splits * (plan.own_slabs ? plan.pieces : 1) * rows64,
                           D, D, f32, 4, 32) &&
             make_tmap_mn(&maps.dz_mn, h->dz, plan.piece, dz_rows, plan.piece) &&
-            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, ldp);
+            make_tmap_mn(&maps.x_mn, h->xp, D, rows64, ldp) &&
+            make_tmap(&maps.twin_k, h->twin, 2 * HB_TWIN, D, ldp, GEMM_BM, 0) &&
+            make_tmap_mn(&maps.twin_mn, h->twin, D, 2 * HB_TWIN, ldp);
   maps.dw_out = maps.dx_out;   // not used without dw
   if (ok && g->dw)
     ok = make_tmap_out(&maps.dw_out, g->dw, V, D, g->lddw, g->dw_f32 ? f32 : bf, esz, 128 / esz);
@@ -726,11 +747,11 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
                           : (plan.pieces - 1) * plan.splits + (last + plan.split_n - 1) / plan.split_n;
     if (g->dx_f32)
       NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
-                         slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx, (int)c.add));
+                         slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx, (int)c.add, (const int*)h->count));
     else
       NE_LAUNCH(launch_k(head_dx_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->st,
                          (const float*)h->dx, slabs, slab, rows, D, (const int*)h->pos_of,
-                         (__nv_bfloat16*)g->dx, g->lddx, 0));
+                         (__nv_bfloat16*)g->dx, g->lddx, 0, (const int*)h->count));
   }
   return NE_OK;
 }
@@ -823,10 +844,11 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   NE_CUDA(cudaStreamSynchronize(ctx->st));
   free_head(ctx);
   const size_t R = n.max_rows, R256 = up(R, 256), D = n.max_dim, V = n.max_vocab;
+  const size_t R64 = std::max<size_t>(up(R, 64), 2 * HB_TWIN);   // few rows stand twice
   const size_t K = std::max(n.max_topk, 1);
   // a piece is at least 256 ids wide, whatever the rows
-  const size_t dz = std::min<size_t>(std::max<size_t>(kPieceBytes, up(R, 64) * HB_BN * 2),
-                                     up(R, 64) * up(V, HB_BN) * 2);
+  const size_t dz = std::min<size_t>(std::max<size_t>(kPieceBytes, R64 * HB_BN * 2),
+                                     R64 * up(V, HB_BN) * 2);
   // pairs of a row: two a tile of at least 192 ids, or two a CTA where there is
   // one tile of rows
   const size_t pairs = std::max(2 * ((V + 191) / 192) * R, (size_t)2 * ctx->num_sms * 2 * GEMM_BM);
@@ -839,9 +861,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4),
                o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
                o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8), o_lse = take(R * 4),
-               o_xp = take(R256 * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
+               o_xp = take(R256 * up(D, GEMM_BK) * 2), o_twin = take(2 * HB_TWIN * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
                o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz = take(HB_BUFS * dz),
-               o_dx = take(std::max(up(R, 64) * D * 4, kSlabBytes)),
+               o_dx = take(std::max(R64 * D * 4, kSlabBytes)),
                o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1) * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
@@ -861,6 +883,7 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   n.stats = (float2*)(b + o_stats);
   n.lse = (float*)(b + o_lse);
   n.xp = (__nv_bfloat16*)(b + o_xp);
+  n.twin = (__nv_bfloat16*)(b + o_twin);
   n.dz = (__nv_bfloat16*)(b + o_dz);
   n.dx = (float*)(b + o_dx);
   n.counters = (int*)(b + o_counters);

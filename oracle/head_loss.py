@@ -62,7 +62,7 @@ def head_loss(x, w, keep, p, plogp, scale=1.0, temperature=1.0, grad=None):
     return loss, lse, dx, scale * (dz.T @ xs)
 
 
-def bounds(x, w, keep, p, scale=1.0, temperature=1.0, grad=None):
+def bounds(x, w, keep, p, scale=1.0, temperature=1.0, grad=None, dz_step=2.0 ** -8):
     """How far the kernels may be from head_loss, entry by entry, by arithmetic:
     returns (loss, lse, dx, dw) bounds without the rounding of the outputs.
 
@@ -74,7 +74,7 @@ def bounds(x, w, keep, p, scale=1.0, temperature=1.0, grad=None):
     chunk sums): e = 2^-17 + 2^-22 |u|max in all.
     lse: du + e, and 2^-22 of its size; loss: T^2 times that and du more.
     dz = a (q - p): q off by q * (2 (du + e)), the value rounded to bf16, half a
-    step, 2^-8 of its size.  dx, dw: those times |w|, |x| summed, and the fp32
+    step, dz_step = 2^-8 of its size (in two parts: 2^-16).  dx, dw: those times |w|, |x| summed, and the fp32
     sums' own 2^-16 of the magnitudes (a step of 16 truncates 2^-23, at most
     a few hundred steps a product here, and one fp32 addition a piece).
     """
@@ -92,7 +92,7 @@ def bounds(x, w, keep, p, scale=1.0, temperature=1.0, grad=None):
     q = torch.softmax(u, 1)
     a = (g[keep].abs() * T * scale)[:, None]
     dz = a * (q - ps).abs()
-    off = a * q * (2 * (du + e)) + 2.0 ** -8 * dz + 2.0 ** -16 * dz + a * 2.0 ** -24
+    off = a * q * (2 * (du + e)) + dz_step * dz + 2.0 ** -16 * dz + a * 2.0 ** -24
     bdx = torch.zeros(x.shape, dtype=torch.float64)
     bdx[keep] = off @ ws.abs()
     return b_loss, b_lse, bdx, off.T @ xs.abs()
