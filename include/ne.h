@@ -399,7 +399,7 @@ NE_API ne_status ne_sdpa_fwd_device(ne_ctx* ctx, const void* d_q, const void* d_
  * All calls only enqueue work on the context's stream, use the workspaces of
  * ne_head_alloc and may be captured into a graph.  dim, ldx, ldw, lddx and
  * lddw are multiples of 8, x, w, dx and dw 16-byte aligned; rows, vocab and
- * topk are arbitrary (rows may be 0).  Outputs must not overlap inputs, and are
+ * topk are arbitrary (rows may be 0, and arrays of rows then NULL).  Outputs must not overlap inputs, and are
  * the same bits every time.  The workspaces belong to one call at a time: graphs
  * of these calls are replayed one after the other.  A target or id >= vocab
  * counts as absent and is reported by the next call that synchronises

@@ -461,8 +461,9 @@ struct HeadCall {
   bool add = false;                     // to loss and dx
 };
 
+// Arrays of no rows may be NULL, as an empty array's address often is.
 ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
-  if (!d->x || !d->w) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x or w is NULL");
+  if ((!d->x && d->rows != 0) || !d->w) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x or w is NULL");
   if (d->rows < 0 || d->dim <= 0 || d->vocab <= 0)
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": rows, dim or vocab out of range");
   if (d->dim % 8) return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": dim must be a multiple of 8");
@@ -480,7 +481,7 @@ ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
 }
 
 ne_status teacher_check(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t, const char* what) {
-  if (!t->ids || !t->logits || t->topk <= 0)
+  if ((d->rows != 0 && (!t->ids || !t->logits)) || t->topk <= 0)
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": teacher ids, logits or topk missing");
   if (t->topk > kTopkMax)
     return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": topk is at most 256");
@@ -757,7 +758,7 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
 }
 
 ne_status grads_check(ne_ctx* ctx, const ne_head_desc* d, const ne_head_grads* g, const char* what) {
-  if (!g->dx && !g->dw) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": no gradient asked for");
+  if (!g->dx && !g->dw && d->rows != 0) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": no gradient asked for");
   if ((g->dx && (g->lddx < d->dim || g->lddx % 8)) || (g->dw && (g->lddw < d->dim || g->lddw % 8)))
     return fail(ctx, NE_ERR_INVALID,
                 std::string(what) + ": lddx and lddw must be multiples of 8, at least dim");
@@ -894,7 +895,7 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
 NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
                                 float* d_loss, float* d_lse) {
   if (!ctx || !d) return NE_ERR_INVALID;
-  if (!d_target || !d_loss || !d_lse)
+  if (d->rows != 0 && (!d_target || !d_loss || !d_lse))
     return fail(ctx, NE_ERR_INVALID, "ne_head_ce_fwd: target, loss or lse is NULL");
   ne_status s = head_check(ctx, d, "ne_head_ce_fwd");
   if (s != NE_OK || d->rows == 0) return s;
@@ -908,7 +909,7 @@ NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_
 NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
                                 const float* d_lse, const float* d_grad, const ne_head_grads* g) {
   if (!ctx || !d || !g) return NE_ERR_INVALID;
-  if (!d_target || !d_lse)
+  if (d->rows != 0 && (!d_target || !d_lse))
     return fail(ctx, NE_ERR_INVALID, "ne_head_ce_bwd: target or lse is NULL");
   ne_status s = head_check(ctx, d, "ne_head_ce_bwd");
   if (s != NE_OK || (s = grads_check(ctx, d, g, "ne_head_ce_bwd")) != NE_OK) return s;
@@ -923,7 +924,7 @@ NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_
 NE_API ne_status ne_head_distill_fwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
                                      float* d_loss, float* d_lse) {
   if (!ctx || !d || !t) return NE_ERR_INVALID;
-  if (!d_loss || !d_lse)
+  if (d->rows != 0 && (!d_loss || !d_lse))
     return fail(ctx, NE_ERR_INVALID, "ne_head_distill_fwd: loss or lse is NULL");
   ne_status s = head_check(ctx, d, "ne_head_distill_fwd");
   if (s != NE_OK || (s = teacher_check(ctx, d, t, "ne_head_distill_fwd")) != NE_OK || d->rows == 0)
@@ -941,7 +942,7 @@ NE_API ne_status ne_head_distill_bwd(ne_ctx* ctx, const ne_head_desc* d, const n
                                      const float* d_lse, const float* d_grad,
                                      const ne_head_grads* g) {
   if (!ctx || !d || !t || !g) return NE_ERR_INVALID;
-  if (!d_lse) return fail(ctx, NE_ERR_INVALID, "ne_head_distill_bwd: lse is NULL");
+  if (d->rows != 0 && !d_lse) return fail(ctx, NE_ERR_INVALID, "ne_head_distill_bwd: lse is NULL");
   ne_status s = head_check(ctx, d, "ne_head_distill_bwd");
   if (s != NE_OK || (s = teacher_check(ctx, d, t, "ne_head_distill_bwd")) != NE_OK ||
       (s = grads_check(ctx, d, g, "ne_head_distill_bwd")) != NE_OK)

@@ -317,6 +317,29 @@ def test_no_rows(eng):
     assert bool((h.dw[:50] == 0.0).all()) and bool((h.dw[50:] == 7.0).all())
 
 
+def test_empty_arrays_have_no_address(eng):
+    """With rows 0 the arrays of rows are NULL; dw of no rows is still written."""
+    eng.head_alloc(1, 64, 50, 4)
+    w = torch.zeros(50, 64, dtype=torch.bfloat16, device="cuda")
+    dw = torch.full((50, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    t = torch.empty(0, 4, dtype=torch.int32, device="cuda")
+    f = torch.empty(0, device="cuda")
+    assert x.data_ptr() == t.data_ptr() == f.data_ptr() == 0
+    torch.cuda.synchronize()
+    head = dict(x=x.data_ptr(), w=w.data_ptr(), rows=0, dim=64, vocab=50)
+    kd = dict(head, ids=t.data_ptr(), teacher=f.data_ptr(), topk=4, lse=f.data_ptr())
+    eng.head_ce_fwd(**head, target=t.data_ptr(), loss=f.data_ptr(), lse=f.data_ptr())
+    eng.head_distill_fwd(**kd, loss=f.data_ptr())
+    eng.head_ce_bwd(**head, target=t.data_ptr(), lse=f.data_ptr(), dx=x.data_ptr())
+    eng.head_distill_bwd(**kd, grad=f.data_ptr(), dx=x.data_ptr())
+    eng.sync()
+    assert bool((dw == 7.0).all())
+    eng.head_ce_bwd(**head, target=t.data_ptr(), lse=f.data_ptr(), dx=x.data_ptr(), dw=dw.data_ptr())
+    eng.sync()
+    assert bool((dw == 0.0).all())
+
+
 def test_captured_and_replayed(eng):
     """Two graphs that share the context's workspaces, replayed in turn with new
     inputs, give what eager calls give."""
