@@ -432,7 +432,8 @@ typedef struct ne_head_grads {
 
 /* Workspaces for calls of up to these sizes (max_topk 0: cross entropy only).
  * A later call with larger sizes waits for the stream and allocates anew, which
- * invalidates graphs captured before; one that fits does nothing. */
+ * invalidates graphs captured before; one that fits does nothing.  Where memory
+ * does not suffice (NE_ERR_OOM) the context has no such workspaces afterwards. */
 NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_vocab, int max_topk);
 
 /* d_loss[i] = lse_i - z[i, target_i], d_lse[i] = log sum_v exp z[i, v] (fp32

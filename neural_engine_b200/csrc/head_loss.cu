@@ -487,8 +487,11 @@ ne_status teacher_check(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_des
     return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": topk is at most 256");
   if (!(t->temperature > 0.f) || !std::isfinite(t->temperature))
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature must be positive and finite");
-  if (!std::isfinite(t->temperature * t->temperature) ||
-      !std::isfinite(d->scale / t->temperature * kLog2e) || !std::isfinite(1.0f / t->temperature))
+  // what the kernels multiply by: an id behind the vocabulary's end counts as -inf
+  // times scale / T, which may not be 0
+  const float u = d->scale / t->temperature * kLog2e;
+  if (!std::isfinite(t->temperature * t->temperature) || !std::isfinite(d->scale * t->temperature) ||
+      !std::isfinite(u) || !(u > 0.f) || !std::isfinite(1.0f / t->temperature))
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature out of range");
   if (t->topk > ctx->head->max_topk)
     return fail(ctx, NE_ERR_STATE, std::string(what) + ": ne_head_alloc has no room for this topk");
@@ -823,6 +826,8 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   if (max_topk > kTopkMax) return fail(ctx, NE_ERR_UNSUPPORTED, "ne_head_alloc: topk is at most 256");
   if (max_rows > (1 << 22))
     return fail(ctx, NE_ERR_UNSUPPORTED, "ne_head_alloc: at most 4194304 rows a call");
+  if (max_dim > (1 << 28) || max_vocab > (1 << 28))   // the kernels count in 32 bits
+    return fail(ctx, NE_ERR_UNSUPPORTED, "ne_head_alloc: dim and vocab are at most 268435456");
   HeadState n;
   n.max_rows = max_rows;
   n.max_dim = max_dim;
@@ -868,7 +873,10 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
                o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1) * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
-  if (s != NE_OK) return s;
+  if (s != NE_OK) {
+    cudaGetLastError();   // reported here, and not by a later launch
+    return s;
+  }
   n.pool = b;
   n.count = (int*)(b + o_count);
   n.row_of = (int*)(b + o_row);

@@ -446,3 +446,38 @@ def test_refusals():
     eng.sync()
     assert bool((h.loss == 7.0).all()) and bool((h.dw == 7.0).all())   # nothing was enqueued
     eng.close()
+
+
+def test_factors_past_the_range_are_refused(eng):
+    """scale / T and scale * T have to be numbers of fp32 other than 0."""
+    import neural_engine_b200 as ne
+    h = Head(4, 64, 100, seed=15).distill(4, 2.0)
+    h.upload()
+    eng.head_alloc(4, 64, 100, 4)
+    for scale, T in ((1e-30, 1e18), (1e30, 1e15)):
+        h.scale, h.T = scale, T
+        with pytest.raises(ne.NeError) as err:
+            eng.head_distill_fwd(**h.head(), ids=h.d_ids.data_ptr(), teacher=h.d_teacher.data_ptr(), topk=4,
+                                 temperature=T, loss=h.loss.data_ptr(), lse=h.lse.data_ptr())
+        assert err.value.status == 1
+
+
+def test_room_that_cannot_be_had():
+    """A size out of range is refused; one that memory cannot hold leaves the
+    context without workspaces and otherwise as it was."""
+    import neural_engine_b200 as ne
+    eng = ne.Engine(ne.ModelConfig(1, 128, 256, 2, 2, 64, 256))
+    for kw in ((1, 2 ** 28 + 8, 10, 0), (1, 64, 2 ** 28 + 1, 0)):
+        with pytest.raises(ne.NeError) as err:
+            eng.head_alloc(*kw)
+        assert err.value.status == 7
+    h = Head(4, 64, 100, seed=16).ce()
+    h.run(eng).check()
+    with pytest.raises(ne.NeError) as err:   # the pairs of the rows alone are 94 TB
+        eng.head_alloc(2 ** 22, 64, 2 ** 28, 0)
+    assert err.value.status == 3
+    with pytest.raises(ne.NeError) as err:
+        h.forward(eng)
+    assert err.value.status == 8
+    h.run(eng).check()
+    eng.close()
