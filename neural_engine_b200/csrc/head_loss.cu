@@ -299,6 +299,11 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
   if (in && !p.keep && !p.pos_of && sl == 0 && p.target[i] >= p.vocab)
     atomicExch(p.status, DEV_ERR_BOUNDS);
   const int m = in && p.pos_of ? p.pos_of[i] : i;
+  // this thread's first entry, on its way while the pairs are joined (with one row
+  // a block it has no other)
+  const bool mine = in && p.keep && sl < p.n;
+  const float q0 = mine ? p.prob[(long long)sl * p.rows + i] : 0.f;
+  const float z0 = mine ? p.zt[(long long)sl * p.rows + i] : 0.f;
   float mx = kLowest, sum = 0.f;
   if (on) {
     const float2* s = p.stats + m * p.row_stride;
@@ -337,7 +342,8 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
   __syncthreads();
   float part = 0.f;
   if (on && p.keep) {
-    for (int k = sl; k < p.n; k += SL) {
+    if (q0 != 0.f) part = q0 * (lse2 - z0);
+    for (int k = sl + SL; k < p.n; k += SL) {
       const float q = p.prob[(long long)k * p.rows + i];
       if (q != 0.f) part += q * (lse2 - p.zt[(long long)k * p.rows + i]);
     }
