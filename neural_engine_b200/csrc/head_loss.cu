@@ -379,19 +379,25 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
   if (at >= (long long)rows * quads) return;
   const int i = (int)(at / quads), k = (int)(at - (long long)i * quads);
   const int pos = pos_of[i];
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool twin = *count <= HB_TWIN;
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 v = zero;
   if (pos >= 0) {
-    const bool twin = *count <= HB_TWIN;
     const float4* src = reinterpret_cast<const float4*>(acc + (long long)pos * dim) + k;
-#pragma unroll 8
-    for (int u = 0; u < slabs; ++u) {
-      const float4 q = src[u * (slab / 4)];
-      v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-      if (twin) {   // the product of dz's second part, 64 rows further
-        const float4 r = src[u * (slab / 4) + HB_TWIN * quads];
-        v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
+    // eight loads in flight, also where fewer are left
+    auto add_slabs = [&](const float4* from) {
+      for (int u0 = 0; u0 < slabs; u0 += 8) {
+        float4 q[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) q[u] = u0 + u < slabs ? from[(u0 + u) * (slab / 4)] : zero;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          v.x += q[u].x; v.y += q[u].y; v.z += q[u].z; v.w += q[u].w;
+        }
       }
-    }
+    };
+    add_slabs(src);
+    if (twin) add_slabs(src + HB_TWIN * quads);   // the products of dz's second part, 64 rows further
   }
   T* dst = dx + (long long)i * ld + 4 * k;
   if constexpr (sizeof(T) == 4) {
