@@ -365,40 +365,56 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
   }
 }
 
-// dx of the rows as the caller laid them out, the slabs added in their order;
-// zeros where a row was left out.  A thread takes four columns.
+// dx of the rows as the caller laid them out, the slabs added in a fixed order;
+// zeros where a row was left out.  A thread takes four columns of up to eight
+// slabs (with more than eight slabs `groups` threads share the columns, and their
+// sums are added in the groups' order): what few rows cost is the chain of loads.
+// Forward and backward pass of 64 rows of 768 columns, 14 slabs that stand twice:
+// 62.5 us, 67.2 without groups.
 template <class T>
 __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int slabs,
-                                                      long long slab, int rows, int dim,
+                                                      long long slab, int rows, int dim, int groups,
                                                       const int* __restrict__ pos_of, T* dx,
                                                       long long ld, int add, const int* count) {
   pdl_trigger();
   pdl_wait();
-  const int quads = dim / 4;
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (long long)rows * quads) return;
+  __shared__ float4 part[256];
+  const int quads = dim / 4, cols = 256 / groups;
+  const int c = threadIdx.x % cols, g = threadIdx.x / cols;
+  const long long at = (long long)blockIdx.x * cols + c;
+  const bool in = at < (long long)rows * quads;
   const int i = (int)(at / quads), k = (int)(at - (long long)i * quads);
-  const int pos = pos_of[i];
-  const bool twin = *count <= HB_TWIN;
+  const int pos = in ? pos_of[i] : -1;
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
   float4 v = zero;
   if (pos >= 0) {
+    // where rows stand twice, the products of dz's second part lie 64 rows further
+    const int all = *count <= HB_TWIN ? 2 * slabs : slabs, each = (all + groups - 1) / groups;
     const float4* src = reinterpret_cast<const float4*>(acc + (long long)pos * dim) + k;
-    // eight loads in flight, also where fewer are left
-    auto add_slabs = [&](const float4* from) {
-      for (int u0 = 0; u0 < slabs; u0 += 8) {
-        float4 q[8];
+    const int end = min(all, (g + 1) * each);
+    for (int u0 = g * each; u0 < end; u0 += 8) {
+      float4 q[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) q[u] = u0 + u < slabs ? from[(u0 + u) * (slab / 4)] : zero;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          v.x += q[u].x; v.y += q[u].y; v.z += q[u].z; v.w += q[u].w;
-        }
+      for (int u = 0; u < 8; ++u) {
+        const int n = u0 + u, second = n >= slabs;
+        q[u] = n < end ? src[(n - second * slabs) * (slab / 4) + second * HB_TWIN * quads] : zero;
       }
-    };
-    add_slabs(src);
-    if (twin) add_slabs(src + HB_TWIN * quads);   // the products of dz's second part, 64 rows further
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        v.x += q[u].x; v.y += q[u].y; v.z += q[u].z; v.w += q[u].w;
+      }
+    }
   }
+  if (groups > 1) {
+    part[threadIdx.x] = v;
+    __syncthreads();
+    if (g > 0) return;
+    for (int u = 1; u < groups; ++u) {
+      const float4 q = part[u * cols + c];
+      v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+    }
+  }
+  if (!in) return;
   T* dst = dx + (long long)i * ld + 4 * k;
   if constexpr (sizeof(T) == 4) {
     if (add) {
@@ -756,19 +772,24 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   if (plan.cg == 2) NE_LAUNCH(launch_walk<2>(maps, walk, dz, plan.clusters, ctx->st));
   else NE_LAUNCH(launch_walk<1>(maps, walk, dz, plan.clusters, ctx->st));
   if (g->dx) {
-    const dim3 grid((unsigned)(((long long)rows * (D / 4) + 255) / 256));
     const long long slab = (long long)rows64 * D;
     // the last piece may have fewer splits than the others
     const int last = V - (plan.pieces - 1) * plan.piece;
     const int slabs = !plan.own_slabs && plan.pieces > 1
                           ? plan.splits
                           : (plan.pieces - 1) * plan.splits + (last + plan.split_n - 1) / plan.split_n;
+    const int loads = rows <= HB_TWIN ? 2 * slabs : slabs;
+    int groups = 1;
+    while (groups < 8 && loads > 8 * groups) groups *= 2;
+    const int cols = 256 / groups;
+    const dim3 grid((unsigned)(((long long)rows * (D / 4) + cols - 1) / cols));
     if (g->dx_f32)
       NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
-                         slabs, slab, rows, D, (const int*)h->pos_of, (float*)g->dx, g->lddx, (int)c.add, (const int*)h->count));
+                         slabs, slab, rows, D, groups, (const int*)h->pos_of, (float*)g->dx, g->lddx,
+                         (int)c.add, (const int*)h->count));
     else
       NE_LAUNCH(launch_k(head_dx_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->st,
-                         (const float*)h->dx, slabs, slab, rows, D, (const int*)h->pos_of,
+                         (const float*)h->dx, slabs, slab, rows, D, groups, (const int*)h->pos_of,
                          (__nv_bfloat16*)g->dx, g->lddx, 0, (const int*)h->count));
   }
   return NE_OK;
