@@ -685,17 +685,18 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
   p.piece = (int)up((vocab + p.pieces - 1) / p.pieces, HB_BN);
   p.pieces = (vocab + p.piece - 1) / p.piece;
   // dx's units are the longest: where there are few of them the piece is split
-  // until a unit is two thirds of what a pair has to do for dx and dw (rows that
-  // do not count make that less than it looks from here), but not below 8 k-blocks,
-  // about what a unit's own hand-over and epilogue cost (19 rows of 2668 ids, forward
-  // and backward: 43.0 us with 8 or 6, 43.8 with 12, 45.4 with 16, 49.0 with 32; calls
+  // until a unit is half of what a pair has to do for dx and dw (64 rows of 32000
+  // ids, forward and backward: 62.5 us with two thirds, 59.8, 60.4 with a third; 256
+  // rows: 70.7, 71.1, 74.3; each split is a slab more to write and read), but not
+  // below 8 k-blocks, about what a unit's own hand-over and epilogue cost (19 rows
+  // of 2668 ids: 43.0 us with 8 or 6, 43.8 with 12, 45.4 with 16, 49.0 with 32; calls
   // with more to do than one unit a pair do not come to it).  dw's units cost 9
   // k-blocks at least, their epilogue.
   const double m_tiles = (double)((rows + p.tile_m - 1) / p.tile_m), d_tiles = (dim + HB_BN - 1) / HB_BN;
   const double piece_kb = p.piece / GEMM_BK;
   const double load = m_tiles * d_tiles * piece_kb +
                       (p.piece / p.tile_m) * d_tiles * std::max(9.0, (double)(rows64 / GEMM_BK));
-  const double most = std::max(8.0, load / p.clusters / 1.5);
+  const double most = std::max(8.0, load / p.clusters / 2);
   const long long slabs = std::max<long long>(1, (long long)kSlabBytes / (rows64 * dim * 4));
   const long long want = std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
   p.split_n = (int)up((p.piece + want - 1) / want, HB_BN);
