@@ -13,12 +13,13 @@
 //     registers over all its tiles.
 // Producers as in head_bwd.cuh: one warp loads A, another B.
 //
-// The tensor cores truncate as they accumulate: a logit's relative error grows
-// by about 4.8e-10 per column of x, always toward zero (measured: lse off by
-// 4.5e-7 at dim 1024, 2.1e-6 at 4096).  Beyond dim 2048 the sum is therefore taken
-// out of tensor memory every 1536 columns and added, rounded to nearest, in
-// registers (LONG): 128 of them a thread, a tile's half row.  2048 rows of 65536
-// ids at dim 4096: 0.88 ms for 0.82, and 6e-7 for 2.1e-6.
+// The tensor cores truncate as they accumulate.  What that loses on average is
+// put back with the factor c2 (logit_factor, head_loss.cu: lse of 925 rows at dim
+// 544 off by 0.9e-7, without it 4.3e-7); what is left of the loss still grows with
+// the columns of a sum (logits at dim 2048: 2.6e-7, of sums of one sign 1.1e-6).
+// Beyond dim 2048 the sum is therefore taken out of tensor memory every 1536
+// columns and added, rounded to nearest, in registers (LONG): 128 of them a
+// thread, a tile's half row.  2048 rows of 65536 ids at dim 4096: 0.88 ms for 0.82.
 #pragma once
 #include "head_bwd.cuh"
 

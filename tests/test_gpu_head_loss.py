@@ -207,6 +207,28 @@ def test_long_sums(eng, rows):
         assert float((h.lse[:rows].cpu().double() - want[1]).abs().max()) <= (1536 * 4.8e-10 + 3 * 2.0 ** -22) * size
 
 
+@pytest.mark.parametrize("rows", [128, 300])
+@pytest.mark.parametrize("dim", [512, 2048, 4096])
+def test_no_bias_from_accumulating(eng, rows, dim):
+    """With one id lse is the logit.  An accumulator that truncates loses half a
+    step of its partial sum in each of dim / 16 additions: of an evenly growing
+    sum ln 2 / 32 * 2^-24 per column (of at most 2048 columns, longer sums are
+    split).  On average less than half of that may be missing or added."""
+    g = torch.Generator().manual_seed(20 + dim)
+    w = torch.randn(1, dim, generator=g).to(torch.bfloat16)
+    x = (0.3 * w.float() + torch.randn(rows, dim, generator=g)).to(torch.bfloat16)
+    z = (x.double() @ w.double().T)[:, 0]
+    d_x, d_w, t = x.cuda(), w.cuda(), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    loss, lse = torch.empty(2, rows, device="cuda")
+    torch.cuda.synchronize()
+    eng.head_alloc(rows, dim, 1)
+    eng.head_ce_fwd(x=d_x.data_ptr(), w=d_w.data_ptr(), rows=rows, dim=dim, vocab=1, target=t.data_ptr(),
+                    loss=loss.data_ptr(), lse=lse.data_ptr())
+    eng.sync()
+    slope = float(((lse.cpu().double() - z) * z).sum() / (z * z).sum())
+    assert abs(slope) < 0.5 * math.log(2) / 32 * 2.0 ** -24 * min(dim, 2048)
+
+
 def test_teacher_entries(eng):
     """Repeats, -inf, ids in any order, NaN and infinity behind absent ids, 256 entries."""
     h = Head(6, 64, 90, seed=5).distill(256, 1.0, ragged=False)
