@@ -253,9 +253,6 @@ __device__ __forceinline__ void head_unit(const HeadWalk& s, const HeadOrder& o,
 __device__ __forceinline__ void flag_add(int* f) {
   asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(f) : "memory");
 }
-__device__ __forceinline__ void flag_add_relaxed(int* f) {
-  asm volatile("red.relaxed.gpu.global.add.s32 [%0], 1;" ::"l"(f) : "memory");
-}
 __device__ __forceinline__ bool flag_reached(const int* f, int want) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
@@ -279,10 +276,11 @@ __device__ __forceinline__ void fence_async_global() {
   asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-// Arrivals and writes across the pair.  The data that crosses is a work unit,
-// written together with its completion (st.async), so nothing has to be
-// fenced at cluster scope: such a release costs an epilogue warp about 1,400
-// cycles, and the matching acquire another 1,000.
+// Arrivals and writes across the pair.  All that crosses is a work unit, written
+// together with its completion (st.async): the hand-over is no release at cluster
+// scope, which would cost an epilogue warp about 1,400 cycles, and the matching
+// acquire another 1,000.  What other SMs wrote is therefore not passed on by it;
+// the peer's A producer acquires the same flags itself (`ready`).
 __device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -493,33 +491,39 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         if (now && !__all_sync(0xffffffffu, flag_wait(f, want, sp.status, abort_flag))) ok = false;
         return now && ok;
       };
-      // hands over the leader's next unit once what it depends on is done: dz,
-      // its buffer was read for the last time; dx and dw, dz was written, and dx
-      // was added to by the piece before.  now: wait for that.
-      auto hand_over = [&](int it, bool now) -> bool {
-        if (nw.kind == HK_DZ) {
-          const int p = nw.piece - HB_BUFS;
+      // What unit w depends on is done: dz, its buffer was read for the last time;
+      // dx and dw, dz was written, and dx was added to by the piece before.  Each
+      // CTA's A producer acquires that itself before it loads or lets the CTA's
+      // epilogue store.  now: wait for it.
+      auto ready = [&](const HeadUnit& w, bool now) -> bool {
+        if (w.kind == HK_DZ) {
+          const int p = w.piece - HB_BUFS;
           if (p > read_to) {
             if (!reached(head_flag(sp, p, HF_READ), ord.full.dx + ord.full.dw, now)) return false;
             read_to = p;
           }
-        } else if (nw.kind != HK_END) {
-          const int split = nw.kind == HK_DX ? nw.split : nw.mt * TILE_M / sp.split_n;
-          if (nw.piece != made_piece || split != made_split) {
-            const int ids = nw.piece == sp.pieces - 1 ? ord.last_ids : sp.piece;
+        } else if (w.kind != HK_END) {
+          const int split = w.kind == HK_DX ? w.split : w.mt * TILE_M / sp.split_n;
+          if (w.piece != made_piece || split != made_split) {
+            const int ids = w.piece == sp.pieces - 1 ? ord.last_ids : sp.piece;
             const int n = (min(ids - split * sp.split_n, sp.split_n) + HB_BN - 1) / HB_BN;
-            if (!reached(head_flag(sp, nw.piece, HF_MADE + split),
+            if (!reached(head_flag(sp, w.piece, HF_MADE + split),
                          n * ord.m_tiles * CG * GEMM_EPI_WARPS, now))
               return false;
-            made_piece = nw.piece;
+            made_piece = w.piece;
             made_split = split;
           }
-          if (nw.kind == HK_DX && !sp.own_slabs && nw.piece - 1 > added_to) {
-            if (!reached(head_flag(sp, nw.piece - 1, HF_ADDED), ord.full.dx * CG * GEMM_EPI_WARPS, now))
+          if (w.kind == HK_DX && !sp.own_slabs && w.piece - 1 > added_to) {
+            if (!reached(head_flag(sp, w.piece - 1, HF_ADDED), ord.full.dx * CG * GEMM_EPI_WARPS, now))
               return false;
-            added_to = nw.piece - 1;
+            added_to = w.piece - 1;
           }
         }
+        return true;
+      };
+      // hands over the leader's next unit once it is ready
+      auto hand_over = [&](int it, bool now) -> bool {
+        if (!ready(nw, now)) return false;
         const int s = it % HB_SLOTS;
         const uint32_t at = slots + 32 * s;
         if (!warp_wait(sempty_bar + 8 * s, ((it / HB_SLOTS) & 1) ^ 1, sp.status, abort_flag)) {
@@ -564,6 +568,7 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
           taken(it);
         }
         if (w.kind == HK_END) break;
+        if (is_a && !leads && !ready(w, true)) break;
         fence_async_global();
         const int buf_row = (w.piece % HB_BUFS) * sp.rows64, id0 = w.piece * sp.piece;
         // this role's operand: K-major is one box, MN-major one per 64 columns
@@ -734,11 +739,11 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       // dz in whole k-blocks of 64 ids: dx's product reads them
       const int cols_end = w.kind == HK_DZ ? (ids + 63) & ~63 : sp.dim;
       // dz has been read, as far as this unit is concerned: its loads arrived
-      // before its products, and nothing this thread wrote has to be ordered (a
-      // release here waits 1,500 to 3,000 cycles for the boxes before).  With no
+      // before its products.  The release waits 1,500 to 3,000 cycles for this
+      // thread's boxes; a piece has then units long enough to hide it.  With no
       // more pieces than buffers nobody asks.
       if (w.kind != HK_DZ && sp.pieces > HB_BUFS && warp == 2 && lane == 0 && crank == 0)
-        flag_add_relaxed(head_flag(sp, w.piece, HF_READ));
+        flag_add(head_flag(sp, w.piece, HF_READ));
       const CUtensorMap* out = w.kind == HK_DZ ? &maps.dz_out
                                : w.kind == HK_DW ? &maps.dw_out : &maps.dx_out;
       // a warp owns half of the tile's columns and sends boxes of 128-byte rows:
