@@ -227,8 +227,10 @@ __global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
   float v = -INFINITY;
   if (k < K) {
     c = ids_in[(long long)r * K + k];
-    v = logit[(long long)r * K + k] * inv_t;
+    const float y = logit[(long long)r * K + k];
+    if (y == -INFINITY) c = -1;   // absent, whatever its id
     if (c >= vocab) atomicExch(status, DEV_ERR_BOUNDS);
+    v = y * inv_t;
   }
   const bool there = c >= 0 && c < vocab && v != -INFINITY;
   if (!there) c = INT_MAX;

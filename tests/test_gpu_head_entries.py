@@ -1,0 +1,33 @@
+"""GPU: a teacher's entries at the edges of what the head losses allow, against
+the float64 definition (tolerances: oracle.head_loss.bounds).
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_head_loss import Head  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+INT_MAX = 2 ** 31 - 1
+
+
+@pytest.fixture()
+def eng():
+    import neural_engine_b200 as ne
+    e = ne.Engine(ne.ModelConfig(1, 128, 256, 2, 2, 64, 256))
+    yield e
+    e.close()
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_ids_behind_a_logit_of_minus_infinity_are_not_looked_at(eng, rows):
+    """Entries padded with -inf and any id are absent, and nothing is reported."""
+    h = Head(rows, 64, 100, seed=rows).distill(6, 2.0, ragged=False)
+    for k, i in enumerate((100, 101, INT_MAX, -1, -2 ** 31)):
+        h.ids[k::5, 1 + k:] = i
+        h.teacher[k::5, 1 + k:] = -math.inf
+    h.ids[3], h.teacher[3] = INT_MAX, -math.inf   # no entry at all
+    h.run(eng).check()
