@@ -215,7 +215,7 @@ __device__ __forceinline__ float block_reduce(float v, float* part, int warps) {
 }
 __global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
     const int32_t* __restrict__ ids_in, const float* __restrict__ logit, int rows, int K, int vocab,
-    float inv_t, int* ids, float* prob, unsigned short* tab, int tab_ld, float* neg_entropy,
+    float temperature, int* ids, float* prob, unsigned short* tab, int tab_ld, float* neg_entropy,
     int* keep, int* status) {
   pdl_trigger();
   pdl_wait();
@@ -227,20 +227,21 @@ __global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
   float v = -INFINITY;
   if (k < K) {
     c = ids_in[(long long)r * K + k];
-    const float y = logit[(long long)r * K + k];
-    if (y == -INFINITY) c = -1;   // absent, whatever its id
+    v = logit[(long long)r * K + k];
+    if (v == -INFINITY) c = -1;   // absent, whatever its id
     if (c >= vocab) atomicExch(status, DEV_ERR_BOUNDS);
-    v = y * inv_t;
   }
-  const bool there = c >= 0 && c < vocab && v != -INFINITY;
+  const bool there = c >= 0 && c < vocab;
   if (!there) c = INT_MAX;
   sid[k] = (unsigned)c;
   const int any = __syncthreads_or(there);
   const float top = block_reduce<true>(there ? v : -INFINITY, part, warps);
-  const float e = there ? expf(v - top) : 0.f;
+  // the differences are divided by T, not the logits: a logit / T may pass the range
+  v = (v - top) / temperature;
+  const float e = there ? expf(v) : 0.f;
   const float sum = block_reduce<false>(e, part, warps);
   const float p = there ? e / sum : 0.f;
-  const float ent = block_reduce<false>(there && p != 0.f ? p * (v - top - logf(sum)) : 0.f, part, warps);
+  const float ent = block_reduce<false>(there && p != 0.f ? p * (v - logf(sum)) : 0.f, part, warps);
   int rank = 0;
 #pragma unroll 4
   for (int j = 0; j < (int)blockDim.x; j += 4) {
@@ -549,8 +550,8 @@ ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
   HeadState* h = ctx->head;
   const int rows = c.d->rows;
   NE_LAUNCH(launch_k(head_teacher_kernel, dim3(rows), dim3((unsigned)up(c.n, 32)), 0, ctx->st,
-                     c.teacher->ids, c.teacher->logits, rows, c.n, c.d->vocab, 1.0f / c.t, h->ids, h->prob, h->tab, tab_entries(c.d->vocab),
-                     h->neg_entropy, h->keep, ctx->d_status));
+                     c.teacher->ids, c.teacher->logits, rows, c.n, c.d->vocab, c.t, h->ids, h->prob,
+                     h->tab, tab_entries(c.d->vocab), h->neg_entropy, h->keep, ctx->d_status));
   return NE_OK;
 }
 

@@ -31,3 +31,21 @@ def test_ids_behind_a_logit_of_minus_infinity_are_not_looked_at(eng, rows):
         h.teacher[k::5, 1 + k:] = -math.inf
     h.ids[3], h.teacher[3] = INT_MAX, -math.inf   # no entry at all
     h.run(eng).check()
+
+
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.parametrize("T", [0.01, 0.5, 1.0, 3.0])
+def test_logits_at_the_ends_of_the_range(eng, T):
+    """A finite logit is an entry however small the temperature: logits / T may pass
+    the range of fp32, their differences from the row's largest decide."""
+    h = Head(8, 64, 100, seed=3).distill(5, T, ragged=False)
+    h.teacher[0] = LOWEST                       # every entry alike: a fifth each
+    h.teacher[1, 1:] = LOWEST                   # one entry has it all
+    h.teacher[2] = -LOWEST                      # a fifth each again
+    h.teacher[3] = torch.tensor([3e38, 2.9e38, 3e38, -3e38, LOWEST])
+    h.teacher[4] = torch.tensor([-3e38, -2.9e38, LOWEST, -math.inf, -2.9e38])
+    h.teacher[5] = 0.0
+    h.teacher[6, ::2] = LOWEST
+    h.run(eng).check()
