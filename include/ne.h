@@ -419,7 +419,7 @@ typedef struct ne_teacher_desc {
   const int32_t* ids;    /* device [rows, topk] */
   const float* logits;   /* device [rows, topk] */
   int topk;
-  float temperature;     /* T > 0: both sides' logits are divided by it */
+  float temperature;     /* T: both sides' logits are divided by it; T^2 is a normal fp32 number */
 } ne_teacher_desc;
 
 /* Gradients to compute (NULL: not computed).  dx [rows, dim] is written, bf16

@@ -533,10 +533,10 @@ ne_status teacher_check(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_des
   if (!(t->temperature > 0.f) || !std::isfinite(t->temperature))
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature must be positive and finite");
   // what the kernels multiply by: an id behind the vocabulary's end counts as -inf
-  // times scale / T, which may not be 0
-  const float u = d->scale / t->temperature * kLog2e;
-  if (!std::isfinite(t->temperature * t->temperature) || !std::isfinite(d->scale * t->temperature) ||
-      !std::isfinite(u) || !(u > 0.f) || !std::isfinite(1.0f / t->temperature))
+  // times scale / T, which may not be 0, and the loss is T^2 times sums that grow
+  // with 1 / T, so T^2 may not lose bits to its exponent
+  const float u = d->scale / t->temperature * kLog2e, t2 = t->temperature * t->temperature;
+  if (!std::isnormal(t2) || !std::isfinite(d->scale * t->temperature) || !std::isfinite(u) || !(u > 0.f))
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": temperature out of range");
   if (t->topk > ctx->head->max_topk)
     return fail(ctx, NE_ERR_STATE, std::string(what) + ": ne_head_alloc has no room for this topk");

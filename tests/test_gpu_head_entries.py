@@ -49,3 +49,24 @@ def test_logits_at_the_ends_of_the_range(eng, T):
     h.teacher[5] = 0.0
     h.teacher[6, ::2] = LOWEST
     h.run(eng).check()
+
+
+def test_temperatures_whose_square_passes_the_range_are_refused(eng):
+    """T^2 is a factor of the loss: at T = 1e-21 it is 0 in fp32, and the loss, of the
+    order of T times the logits, was too."""
+    import neural_engine_b200 as ne
+    h = Head(4, 64, 100, seed=15).distill(4, 2.0)
+    h.upload()
+    eng.head_alloc(4, 64, 100, 4)
+    for T in (1e-21, 5e-20, 2e19):
+        h.T = T
+        kd = dict(h.head(), ids=h.d_ids.data_ptr(), teacher=h.d_teacher.data_ptr(), topk=4, temperature=T,
+                  lse=h.lse.data_ptr())
+        for call in (lambda: eng.head_distill_fwd(**kd, loss=h.loss.data_ptr()),
+                     lambda: eng.head_distill_bwd(**kd, dx=h.dx.data_ptr(), dw=h.dw.data_ptr())):
+            with pytest.raises(ne.NeError) as err:
+                call()
+            assert err.value.status == 1
+    eng.sync()
+    assert bool((h.loss == 7.0).all()) and bool((h.dw == 7.0).all())
+    Head(4, 64, 100, seed=16).distill(4, 2e-6).run(eng)   # far from it
