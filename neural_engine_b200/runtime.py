@@ -16,7 +16,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libne.so")
 
 # ne_status values (include/ne.h)
-NE_OK = 0
+NE_OK, NE_ERR_INVALID = 0, 1
 STATUS_NAMES = {0: "NE_OK", 1: "NE_ERR_INVALID", 2: "NE_ERR_CUDA", 3: "NE_ERR_OOM",
                 4: "NE_ERR_IO", 5: "NE_ERR_FORMAT", 6: "NE_ERR_TIMEOUT",
                 7: "NE_ERR_UNSUPPORTED", 8: "NE_ERR_STATE", 9: "NE_ERR_BOUNDS"}
@@ -264,6 +264,14 @@ def _ptr(a: np.ndarray | None):
     return a.ctypes.data_as(C.c_void_p)
 
 
+def _c_int(n, name: str) -> int:
+    """A size for a C int: ctypes drops the bits above 32 without a word."""
+    n = int(n)
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise NeError(NE_ERR_INVALID, f"{name} = {n} is out of range")
+    return n
+
+
 class Engine:
     """One GPU context of libne.so (one model, its weights and KV cache)."""
 
@@ -345,7 +353,7 @@ class Engine:
                                d_loss: int | None = None):
         """lmhead_ce_fwd_bwd with a teacher's top logits (device [B*S, topk] ids and logits):
         (1 - hard_weight) * distillation + hard_weight * cross entropy; needs head_alloc."""
-        t = TeacherDescC(ids, teacher, topk, temperature)
+        t = self._teacher(ids, teacher, topk, temperature)
         self._check(self.lib.ne_lmhead_distill_fwd_bwd(self._ctx, C.byref(t) if ids else None,
                                                        hard_weight, d_loss))
 
@@ -368,12 +376,18 @@ class Engine:
     #    distillation from x [rows, dim] and w [vocab, dim], logits never kept
     def head_alloc(self, max_rows: int, max_dim: int, max_vocab: int, max_topk: int = 0):
         """Room for head-loss calls of up to these sizes (max_topk 0: cross entropy only)."""
-        self._check(self.lib.ne_head_alloc(self._ctx, int(max_rows), int(max_dim), int(max_vocab),
-                                           int(max_topk)))
+        self._check(self.lib.ne_head_alloc(
+            self._ctx, _c_int(max_rows, "max_rows"), _c_int(max_dim, "max_dim"),
+            _c_int(max_vocab, "max_vocab"), _c_int(max_topk, "max_topk")))
 
     @staticmethod
     def _head(x, w, rows, dim, vocab, scale, ldx, ldw):
+        rows, dim, vocab = _c_int(rows, "rows"), _c_int(dim, "dim"), _c_int(vocab, "vocab")
         return HeadDescC(x, ldx or dim, w, ldw or dim, rows, dim, vocab, scale)
+
+    @staticmethod
+    def _teacher(ids, teacher, topk, temperature):
+        return TeacherDescC(ids, teacher, _c_int(topk, "topk"), temperature)
 
     @staticmethod
     def _head_grads(dim, dx, dw, lddx, lddw, dx_f32, dw_f32):
@@ -400,7 +414,7 @@ class Engine:
         """Row losses T^2 KL(teacher's topk || softmax(z / T)) and log-sum-exps of z / T; an
         entry with id < 0 is absent, a row without entries is left out."""
         d = self._head(x, w, rows, dim, vocab, scale, ldx, ldw)
-        t = TeacherDescC(ids, teacher, topk, temperature)
+        t = self._teacher(ids, teacher, topk, temperature)
         self._check(self.lib.ne_head_distill_fwd(self._ctx, C.byref(d), C.byref(t), loss, lse))
 
     def head_distill_bwd(self, x: int, w: int, rows: int, dim: int, vocab: int, ids: int,
@@ -410,7 +424,7 @@ class Engine:
                          lddw: int = 0, dx_f32: bool = False, dw_f32: bool = False):
         """Gradients of sum(grad * loss) of head_distill_fwd, as head_ce_bwd gives them."""
         d = self._head(x, w, rows, dim, vocab, scale, ldx, ldw)
-        t = TeacherDescC(ids, teacher, topk, temperature)
+        t = self._teacher(ids, teacher, topk, temperature)
         g = self._head_grads(dim, dx, dw, lddx, lddw, dx_f32, dw_f32)
         self._check(self.lib.ne_head_distill_bwd(self._ctx, C.byref(d), C.byref(t), lse, grad,
                                                  C.byref(g)))
