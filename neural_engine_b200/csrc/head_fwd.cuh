@@ -13,13 +13,15 @@
 //     registers over all its tiles.
 // Producers as in head_bwd.cuh: one warp loads A, another B.
 //
-// The tensor cores truncate as they accumulate.  What that loses on average is
-// put back with the factor c2 (logit_factor, head_loss.cu: lse of 925 rows at dim
-// 544 off by 0.9e-7, without it 4.3e-7); what is left of the loss still grows with
-// the columns of a sum (logits at dim 2048: 2.6e-7, of sums of one sign 1.1e-6).
-// Beyond dim 2048 the sum is therefore taken out of tensor memory every 1536
-// columns and added, rounded to nearest, in registers (LONG): 128 of them a
-// thread, a tile's half row.  2048 rows of 65536 ids at dim 4096: 0.88 ms for 0.82.
+// The tensor cores truncate as they accumulate: each addition of 16 products
+// loses up to 2^-23 of the partial sum (on average 0.8e-9 to 1.6e-9 of the logit
+// per column; nothing where the sum is exact).  So a sum stays in tensor memory for
+// at most 384 columns and is added, rounded to nearest, in registers (LONG): 128 of
+// them a thread, a tile's half row.  Off by, of the logit at dim 2048: random signs
+// 3.6e-7, one sign 5.3e-7, exact sums 0, large products first 1.4e-6 (in one sum
+// 1.9e-6, 5.6e-6, 0, 1.1e-5).  4096 rows of 32000 ids at dim 768: 142 us
+// (one sum of 768: 140), 50000 ids at dim 1024: 273 (271), at dim 512: 175 (148, two
+// runs are shorter than a tile's epilogue); one token of 32000 ids: 14.2 (14.2).
 #pragma once
 #include "head_bwd.cuh"
 
@@ -27,8 +29,7 @@ namespace ne {
 
 constexpr int HF_MAX_STAGES = 12;
 constexpr int HF_HINT_KB = 16;
-constexpr int HF_LONG_KB = 24;   // k-blocks of 64 between two takings (LONG)
-constexpr int HF_LONG_FROM = 32;
+constexpr int HF_RUN_KB = 6;   // k-blocks of 64 a sum stays in tensor memory for, at most
 
 struct HeadLse {
   HeadTargets t;
@@ -40,6 +41,7 @@ struct HeadLse {
   float c2;              // scale / (T ln 2)
   int rows, vocab, dim_kb;
   int bn, n_tiles, group_m;
+  int run_kb;            // k-blocks of 64 that a sum stays in tensor memory for (LONG)
   int a_rows, stages;    // rows of a box of x; ring depth
   int one_row_tile;      // all units have the same rows: one pair per CTA
 };
@@ -84,6 +86,45 @@ __device__ __forceinline__ void lse_chunk(const HeadLse& p, LseRow& r, TargetCur
       p.zt[cur.at * p.t.ld + cur.row] = z * p.c2;
     }
     cursor_step<false>(p.t, cur);
+  }
+}
+
+// The same of a warp's half of a tile, four chunks of 32 columns 64 apart that are
+// all in registers: one maximum for all (4096 rows of 50000 ids at dim 512: 175 us,
+// chunk by chunk 184).
+__device__ __forceinline__ void lse_half(const HeadLse& p, LseRow& r, TargetCursor& cur, float (&v)[4][32],
+                                         int n0, int n_end) {
+  if (n0 + 224 > n_end) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (n0 + 64 * g + j >= n_end) v[g][j] = -INFINITY;
+  }
+  float t4[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+#pragma unroll
+  for (int j = 4; j < 128; ++j) t4[j & 3] = fmaxf(t4[j & 3], v[j >> 5][j & 31]);
+  const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+  const float nm = fmaxf(r.mx, top * p.c2);
+  float s4[4] = {r.sum * ex2_fast(r.mx - nm), 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 128; ++j) s4[j & 3] += ex2_fast(fmaf(v[j >> 5][j & 31], p.c2, -nm));
+  r.mx = nm;
+  r.sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int first = n0 + 64 * g, stop = min(first + 32, n_end);
+    while (cur.next < stop) {
+      if (cur.next >= first) {
+        const int j = cur.next - first;
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i == j) z = v[g][i];
+        p.zt[cur.at * p.t.ld + cur.row] = z * p.c2;
+      }
+      cursor_step<false>(p.t, cur);
+    }
   }
 }
 
@@ -214,11 +255,11 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
       uint32_t acc_phase = 0;
       bool ok = true;
       for (int u = cluster; u < units && ok; u += clusters) {
-        for (int k0 = 0; k0 < p.dim_kb && ok; k0 += LONG ? HF_LONG_KB : p.dim_kb) {
+        for (int k0 = 0; k0 < p.dim_kb && ok; k0 += LONG ? p.run_kb : p.dim_kb) {
           if (!warp_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, p.status, abort_flag)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + acc * HB_BN;
-          const int kn = LONG ? min(HF_LONG_KB, p.dim_kb - k0) : p.dim_kb;
+          const int kn = LONG ? min(p.run_kb, p.dim_kb - k0) : p.dim_kb;
           for (int k = 0; k < kn; ++k) {
             if (!warp_wait(full_bar + 8 * stage, phase, p.status, abort_flag)) { ok = false; break; }
             tc_fence_after();
@@ -285,24 +326,30 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
       const int n_tile = nt * p.bn, n_end = min(n_tile + p.bn, p.vocab);
       const bool has_rows = m - lane < M;   // the warp's
       TargetCursor cur;
-      cursor_seek<false>(p.t, cur, m, M, n_tile);
       if (!p.one_row_tile) r = none;
       if constexpr (LONG) {
         float sum[4][32];
         bool ok = true;
-        for (int k = 0; k < p.dim_kb; k += HF_LONG_KB) {
+#pragma unroll 1
+        for (int k = 0; k < p.dim_kb; k += p.run_kb) {
+          // a chain of loads: behind the tile's first loads of w where those are the
+          // bound, else behind the MMAs of its last run
+          if (p.one_row_tile ? k == 0 : k + p.run_kb >= p.dim_kb) cursor_seek<false>(p.t, cur, m, M, n_tile);
           if (!acquire()) { ok = false; break; }
           if (has_rows) {
+            const uint32_t t = t_lane + acc * HB_BN + 32 * half;
+            if (k == 0) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int c = 32 * half + 64 * g;
-              if (c >= p.bn) continue;
+              for (int g = 0; g < 4; ++g) tmem_ld32_issue(t + 64 * g, sum[g]);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float v[16];
-                tmem_ld16(t_lane + acc * HB_BN + c + 16 * h, v);
+              for (int g = 0; g < 4; ++g) tmem_ld32_wait(sum[g]);
+            } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) sum[g][16 * h + j] = k ? sum[g][16 * h + j] + v[j] : v[j];
+              for (int g = 0; g < 4; ++g) {
+                float v[32];
+                tmem_ld32(t + 64 * g, v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[g][j] += v[j];
               }
             }
           }
@@ -310,13 +357,18 @@ head_lse_kernel(const __grid_constant__ CUtensorMap x_k, const __grid_constant__
         }
         if (!ok) break;
         if (has_rows) {
+          if constexpr (PAIR) {
+            lse_half(p, r, cur, sum, n_tile + 32 * half, n_end);
+          } else {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int n0 = n_tile + 32 * half + 64 * g;
-            if (n0 < n_end) lse_chunk(p, r, cur, sum[g], n0, n_end);
+            for (int g = 0; g < 4; ++g) {
+              const int n0 = n_tile + 32 * half + 64 * g;
+              if (n0 < n_end) lse_chunk(p, r, cur, sum[g], n0, n_end);
+            }
           }
         }
       } else {
+        cursor_seek<false>(p.t, cur, m, M, n_tile);
         if (!acquire()) break;
         if (has_rows) {
 #pragma unroll 1

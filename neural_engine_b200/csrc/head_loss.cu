@@ -483,17 +483,8 @@ int raster_group(int rows, int dim, int tile_m) {
   return panel * m_tiles > budget ? (int)std::max<long long>(1, budget / panel) : 0;
 }
 
-// What turns an accumulated logit into log2 units of the softmax.  The tensor
-// cores truncate: of the dim / 16 additions that make a logit each loses half a
-// step of the partial sum on average, which for sums that grow evenly is
-// ln 2 / 32 * 2^-24 = 1.3e-9 of the logit per column added (measured, dim 128 to
-// 2048: 0.8e-9 for random signs, 1.0e-9 to 1.6e-9 the more of one sign).  1.1e-9 is
-// put back.  Sums taken out every `run` columns lose by the columns of their run.
-float logit_factor(float scale, float t, int dim, int run) {
-  double sq = 0;
-  for (int k = 0; k < dim; k += run) sq += (double)std::min(run, dim - k) * std::min(run, dim - k);
-  return (float)((double)scale / t * 1.4426950408889634 * (1 + 1.1e-9 * sq / dim));
-}
+// What turns a logit into log2 units of the softmax.
+float logit_factor(float scale, float t) { return (float)((double)scale / t * 1.4426950408889634); }
 
 // What a call works on, after its arguments were checked.
 struct HeadCall {
@@ -628,7 +619,9 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   const int parts = 2 * (plan.one_row_tile ? (int)std::min<long long>(units, plan.clusters) : n_tiles);
   HeadLse p{};
   p.dim_kb = (D + GEMM_BK - 1) / GEMM_BK;
-  const bool lng = p.dim_kb > HF_LONG_FROM;   // long sums (head_fwd.cuh)
+  const int runs = (p.dim_kb + HF_RUN_KB - 1) / HF_RUN_KB;
+  p.run_kb = (p.dim_kb + runs - 1) / runs;
+  const bool lng = runs > 1;
   p.t = targets_of(h, c, plan.packed);
   p.d_rows = plan.packed ? h->count : nullptr;
   p.status = ctx->d_status;
@@ -636,7 +629,7 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   p.part_stride = plan.one_row_tile ? 1 : rows;
   p.row_stride = plan.one_row_tile ? parts : 1;
   p.zt = h->zt;
-  p.c2 = logit_factor(d.scale, c.t, D, lng ? HF_LONG_KB * GEMM_BK : D);
+  p.c2 = logit_factor(d.scale, c.t);
   p.rows = rows;
   p.vocab = V;
   p.bn = plan.bn;
@@ -750,7 +743,7 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   HeadDz dz{};
   dz.t = targets_of(h, c, true);
   dz.coef = h->coef;
-  dz.c2 = logit_factor(d.scale, c.t, D, D);
+  dz.c2 = logit_factor(d.scale, c.t);
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const long long ldp = (long long)up(D, GEMM_BK);
   const int esz = g->dw_f32 ? 4 : 2, dz_rows = HB_BUFS * rows64;
