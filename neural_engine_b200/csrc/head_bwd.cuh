@@ -17,6 +17,12 @@
 // whatever the number of CTAs that run; it is bounded all the same.  Which pair
 // computes a unit changes no value: every unit is computed whole, and dx adds
 // the pieces in their order.
+// The tensor cores truncate as they add (head_fwd.cuh), so a unit of more than 1024
+// products a sum is taken out of tensor memory in runs, which are added in registers:
+// fp32 dw of 400000 rows of one sign was 1e-3 too small in one sum, and at dim 4096
+// logits summed otherwise than the forward pass's put gradients of few rows 9e-4 off
+// (1e-4 in runs).  It costs 1 to 2% (4096 rows of 151936 ids, forward and backward:
+// 4.06 -> 4.13 ms, 256 rows of 32000 ids 74.2 -> 75.3 us).
 // As launches of their own the products left 14% of the pairs idle in their last
 // waves (4096 rows, dim 1024: 64 tiles of dx, 128 of dw, for 74 pairs).
 //
@@ -32,6 +38,7 @@ namespace ne {
 constexpr int HB_BN = 256;
 constexpr int HB_SLOTS = 8;
 constexpr int HB_DRAW = 12, HB_TAKE = 6;        // k-blocks before a unit's end
+constexpr int HB_RUN_KB = 16;                   // k-blocks that a sum stays in tensor memory for, at most
 constexpr int HB_THREADS = GEMM_THREADS + 32;   // warps: A, MMA, 8 x epilogue, B
 constexpr int HB_BOX = 4096;                    // 32 rows of 128 bytes
 constexpr int HB_TWIN = 64;                     // up to here rows stand twice
@@ -174,6 +181,12 @@ struct FastDiv {
     return (int)q;
   }
 };
+
+// A unit is summed in equal runs: the k-blocks of one.
+__device__ __forceinline__ int unit_run(const HeadUnit& w) {
+  const int runs = (w.kb + HB_RUN_KB - 1) / HB_RUN_KB;
+  return runs < 2 ? w.kb : (w.kb + runs - 1) / runs;
+}
 
 // What the walk is made of, derived once from the number of rows.
 struct HeadOrder {
@@ -374,6 +387,25 @@ __device__ __forceinline__ void tmem_ld32_wait(float (&v)[32]) {
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   tmem_ld32_issue(taddr, v);
   tmem_ld32_wait(v);
+}
+
+// Back to tensor memory: 32 columns of this lane's row, there after tmem_st_wait.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      :
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]),
+        "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]),
+        "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]),
+        "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+        "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]),
+        "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 template <int CG>
@@ -647,39 +679,44 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         if (!take(it, w)) break;
         taken(it);
         if (w.kind == HK_END) break;
-        if (!warp_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, sp.status, abort_flag)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * HB_BN;
         const int a_mn = w.kind == HK_DW, b_mn = w.kind != HK_DZ;
         const uint32_t idesc = umma_idesc_f16(TILE_M, w.n, 1) | ((uint32_t)a_mn << 15) |
                                ((uint32_t)b_mn << 16);
         const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+        const int run = unit_run(w);
         bool ok = true;
-        for (int k = 0; k < w.kb; ++k) {
-          if (!warp_wait(full_bar + 8 * stage, phase, sp.status, abort_flag)) { ok = false; break; }
+        for (int k0 = 0; k0 < w.kb && ok; k0 += run) {
+          if (!warp_wait(tempty_bar + 8 * acc, acc_phase ^ 1u, sp.status, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          if (elect_one()) {
-            const uint32_t sa = tiles + stage * C::STAGE_BYTES;
-            const uint64_t ad = a_mn ? smem_desc_mn_sw128(sa, MN_BOX) : smem_desc_k_sw128(sa);
-            const uint64_t bd = b_mn ? smem_desc_mn_sw128(sa + C::A_BYTES, MN_BOX)
-                                     : smem_desc_k_sw128(sa + C::A_BYTES);
+          const uint32_t d_tmem = tmem_base + acc * HB_BN;
+          const int kn = min(run, w.kb - k0);
+          for (int k = 0; k < kn; ++k) {
+            if (!warp_wait(full_bar + 8 * stage, phase, sp.status, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t sa = tiles + stage * C::STAGE_BYTES;
+              const uint64_t ad = a_mn ? smem_desc_mn_sw128(sa, MN_BOX) : smem_desc_k_sw128(sa);
+              const uint64_t bd = b_mn ? smem_desc_mn_sw128(sa + C::A_BYTES, MN_BOX)
+                                       : smem_desc_k_sw128(sa + C::A_BYTES);
 #pragma unroll
-            for (int j = 0; j < GEMM_BK / 16; ++j)
-              if constexpr (PAIR)
-                umma_f16_pair(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
-              else
-                umma_f16(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
-            if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
-            else umma_commit(empty_bar + 8 * stage);
+              for (int j = 0; j < GEMM_BK / 16; ++j)
+                if constexpr (PAIR)
+                  umma_f16_pair(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
+                else
+                  umma_f16(d_tmem, ad + a_step * j, bd + b_step * j, idesc, (k | j) != 0);
+              if constexpr (PAIR) umma_commit_pair(empty_bar + 8 * stage, 0x3);
+              else umma_commit(empty_bar + 8 * stage);
+            }
+            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           }
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (!ok) break;
+          if (elect_one()) {
+            if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
+            else umma_commit(tfull_bar + 8 * acc);
+          }
+          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
         }
         if (!ok) break;
-        if (elect_one()) {
-          if constexpr (PAIR) umma_commit_pair(tfull_bar + 8 * acc, 0x3);
-          else umma_commit(tfull_bar + 8 * acc);
-        }
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
       if (elect_one()) {
         if constexpr (PAIR) umma_commit_pair(drain_bar, 0x1);
@@ -709,6 +746,22 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         owed = nullptr;
       }
     };
+    // waits for the accumulator and gives it back
+    auto acquire = [&]() -> bool {
+      if (lane == 0 && owed && !mbar_try_wait(tfull_bar + 8 * acc, acc_phase)) settle();
+      if (!warp_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag)) return false;
+      tc_fence_after();
+      return true;
+    };
+    auto release = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_peer(mapa_shared(tempty_bar + 8 * acc, 0));
+        else mbar_arrive(tempty_bar + 8 * acc);
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    };
     for (int it = 0;; ++it) {
       if (lane == 0 && owed && !mbar_try_wait(sfull_bar + 8 * (it % HB_SLOTS), (it / HB_SLOTS) & 1))
         settle();
@@ -736,77 +789,47 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         }
         cursor_seek<true>(dzp.t, cur, m, count, id0 + n_tile + 128 * half);
       }
-      if (lane == 0 && owed && !mbar_try_wait(tfull_bar + 8 * acc, acc_phase)) settle();
-      if (!warp_wait(tfull_bar + 8 * acc, acc_phase, sp.status, abort_flag)) break;
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * HB_BN;
+      const uint32_t t_half = tmem_base + ((uint32_t)(quarter * 32) << 16) + 128 * half;
       const bool b16 = w.kind == HK_DZ || (w.kind == HK_DW && !sp.dw_f32);
       const bool rows_in = y0 < (w.kind == HK_DW ? ids : M);
       // dz in whole k-blocks of 64 ids: dx's product reads them
       const int cols_end = w.kind == HK_DZ ? (ids + 63) & ~63 : sp.dim;
-      // dz has been read, as far as this unit is concerned: its loads arrived
-      // before its products.  The release waits 1,500 to 3,000 cycles for this
-      // thread's boxes; a piece has then units long enough to hide it.  With no
-      // more pieces than buffers nobody asks.
-      if (w.kind != HK_DZ && sp.pieces > HB_BUFS && warp == 2 && lane == 0 && crank == 0)
-        flag_add(head_flag(sp, w.piece, HF_READ));
       const CUtensorMap* out = w.kind == HK_DZ ? &maps.dz_out
                                : w.kind == HK_DW ? &maps.dw_out : &maps.dx_out;
-      // a warp owns half of the tile's columns and sends boxes of 128-byte rows:
-      // 64 columns of bf16 or 32 of fp32 at a time
-      const int step = b16 ? 64 : 32;
       const bool add = w.kind == HK_DX ? w.piece > 0 && !sp.own_slabs : w.kind == HK_DW && sp.dw_f32;
       const int y = y0 + (w.kind == HK_DX ? (w.split + (sp.own_slabs ? w.piece * sp.splits : 0)) * sp.rows64
                           : w.kind == HK_DW ? id0 : (w.piece % HB_BUFS) * sp.rows64);
-#pragma unroll 1
-      for (int c = 128 * half; c < 128 * half + 128; c += step) {
-        const int n0 = n_tile + c;
-        if (n0 >= cols_end) break;
-        uint32_t o[32];
-        if (b16) {
+      const int n_half = n_tile + 128 * half;
+      // 32 logits of columns n0 .. to dz.
+      // dz is rounded once to bf16 by pack_bf16: it is the operand of two tensor-core
+      // products.  Where rows stand twice, the second 64 take what the rounding of
+      // the first leaves: with few rows the error of one large dz (a target's) does
+      // not average out
+      auto to_dz = [&](float (&v)[32], int n0) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v[32];
-            tmem_ld32(t_row + c + 32 * h, v);
-            if (w.kind == HK_DZ) {
+        for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
+        if (n0 + 32 > ids) {   // behind the last id of the vocabulary
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
-              if (n0 + 32 * h + 32 > ids) {   // behind the last id of the vocabulary
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (n0 + 32 * h + j >= ids) v[j] = 0.f;
-              }
-              const int col = id0 + n0 + 32 * h;
-              while (cur.next < col + 32) {
-                if (cur.next >= col) {
-                  const int j = cur.next - col;
-#pragma unroll
-                  for (int i = 0; i < 32; ++i)
-                    if (i == j) v[i] -= mag * cur.q;
-                }
-                cursor_step<true>(dzp.t, cur);
-              }
-            }
-            // rounded once to bf16: dz is the operand of two tensor-core
-            // products, dw the caller's type.  Where rows stand twice, the second
-            // 64 take what the rounding of the first leaves: with few rows the
-            // error of one large dz (a target's) does not average out
-            if (w.kind == HK_DZ && twin && y0 >= HB_TWIN) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
-            }
-            pack_bf16(v, o + 16 * h);
-          }
-          if (w.kind == HK_DZ) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
-          }
-        } else {
-          float v[32];
-          tmem_ld32(t_row + c, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
+          for (int j = 0; j < 32; ++j)
+            if (n0 + j >= ids) v[j] = 0.f;
         }
+        const int col = id0 + n0;
+        while (cur.next < col + 32) {
+          if (cur.next >= col) {
+            const int j = cur.next - col;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i == j) v[i] -= mag * cur.q;
+          }
+          cursor_step<true>(dzp.t, cur);
+        }
+        if (twin && y0 >= HB_TWIN) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+        }
+      };
+      // sends a box of 128-byte rows: 64 columns of bf16 or 32 of fp32 from column n0
+      auto send = [&](const uint32_t (&o)[32], int n0) {
         if (lane == 0) {   // the previous box has left the slot
           if (owed) settle();
           else bulk_wait_read_all();
@@ -822,20 +845,73 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
           }
           bulk_commit_group();
         }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_peer(mapa_shared(tempty_bar + 8 * acc, 0));
-        else mbar_arrive(tempty_bar + 8 * acc);
-        // others wait for what this unit wrote
-        if (w.kind != HK_DW) {
-          if (owed) settle();   // a unit without a box of its own
-          owed = head_flag(sp, w.piece,
-                           w.kind == HK_DZ ? HF_MADE + w.nt * HB_BN / sp.split_n : HF_ADDED);
+      };
+      const int run = unit_run(w);
+      if (run < w.kb) {
+        // runs before the last are added, rounded to nearest, in registers (128 of
+        // them, this lane's half row), and then to the last one's accumulator
+        float sum[4][32];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[g][j] = 0.f;
+        bool ok = true;
+#pragma unroll 1
+        for (int k = 0; k < w.kb; k += run) {
+          if (!acquire()) { ok = false; break; }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float v[32];
+            tmem_ld32(t_half + acc * HB_BN + 32 * g, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[g][j] += v[j];
+          }
+          if (k + run < w.kb) release();
         }
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) tmem_st32(t_half + acc * HB_BN + 32 * g, sum[g]);
+        tmem_st_wait();
+      } else if (!acquire()) {
+        break;
       }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      // dz has been read, as far as this unit is concerned: its loads arrived
+      // before its products.  The release waits 1,500 to 3,000 cycles for this
+      // thread's boxes; a piece has then units long enough to hide it.  With no
+      // more pieces than buffers nobody asks.
+      if (w.kind != HK_DZ && sp.pieces > HB_BUFS && warp == 2 && lane == 0 && crank == 0)
+        flag_add(head_flag(sp, w.piece, HF_READ));
+#pragma unroll 1
+      for (int c = 0; c < 128; c += b16 ? 64 : 32) {
+        if (n_half + c >= cols_end) break;
+        uint32_t o[32];
+        if (b16) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            tmem_ld32(t_half + acc * HB_BN + c + 32 * h, v);
+            if (w.kind == HK_DZ) to_dz(v, n_half + c + 32 * h);
+            pack_bf16(v, o + 16 * h);
+          }
+          if (w.kind == HK_DZ) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = (o[j] ^ sign) & keep;
+          }
+        } else {
+          float v[32];
+          tmem_ld32(t_half + acc * HB_BN + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j]);
+        }
+        send(o, n_half + c);
+      }
+      release();
+      // others wait for what this unit wrote
+      if (lane == 0 && w.kind != HK_DW) {
+        if (owed) settle();   // a unit without a box of its own
+        owed = head_flag(sp, w.piece,
+                         w.kind == HK_DZ ? HF_MADE + w.nt * HB_BN / sp.split_n : HF_ADDED);
+      }
     }
     if (lane == 0) settle();
   }

@@ -88,3 +88,52 @@ def test_sums_lose_by_their_runs(eng, rows, dim, kind):
     err = (_logits(eng, x, w) - z).abs()
     bound = (24 * 5.25 * 2.0 ** -23 + runs * 2.0 ** -24) * mag + REL * z.abs() + ABS
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+def _gradients(eng, x, w, target, f32, dx=False):
+    """dx or dw of sum of the losses: fp32 (dw added to zeros) or bf16, as float64."""
+    (rows, dim), vocab = x.shape, w.shape[0]
+    loss, lse = torch.empty(2, rows, device="cuda")
+    out = torch.zeros(x.shape if dx else w.shape, dtype=torch.float32 if f32 else torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    head = dict(x=x.data_ptr(), w=w.data_ptr(), rows=rows, dim=dim, vocab=vocab, target=target.data_ptr(),
+                lse=lse.data_ptr())
+    eng.head_alloc(rows, dim, vocab)
+    eng.head_ce_fwd(**head, loss=loss.data_ptr())
+    eng.head_ce_bwd(**head, **{"dx" if dx else "dw": out.data_ptr(), "dx_f32" if dx else "dw_f32": f32})
+    eng.sync()
+    return out.double()
+
+
+# A run of a gradient's sum is 1024 products at most, 64 additions (see
+# test_sums_lose_by_their_runs), and the runs are added in fp32.
+def _bound(n, mag):
+    return (64 * 5.25 * 2.0 ** -23 + (n / 1024 + 1) * 2.0 ** -24) * mag
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("rows", [1000, 1024, 1025, 5000, 400000])
+def test_dw_of_many_rows_of_one_sign(eng, rows, f32):
+    """w = 0 and two ids: every dz is a half, which bf16 holds, so the sums over the
+    rows are all that rounds."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.rand(rows, 72, generator=g, device="cuda").to(torch.bfloat16)
+    got = _gradients(eng, x, torch.zeros(2, 72, dtype=torch.bfloat16, device="cuda"),
+                     torch.ones(rows, dtype=torch.int32, device="cuda"), f32)
+    half = 0.5 * x.double().sum(0)
+    off = (got - torch.stack([half, -half])).abs()
+    assert bool((off <= _bound(rows, half) + (0.0 if f32 else 2.0 ** -8) * half).all()), float((off / half).max())
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("rows,dim", [(200, 72), (4096, 72), (2048, 1024)])
+def test_dx_of_many_ids_of_one_sign(eng, rows, dim, f32):
+    """x = 0 and 2^17 ids: every dz is 2^-17 but the target's, whose row of w is 0."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    w = torch.rand(1 << 17, dim, generator=g, device="cuda").to(torch.bfloat16)
+    target = torch.randint(0, 1 << 17, (rows,), generator=g, device="cuda").to(torch.int32)
+    w[target.long()] = 0
+    got = _gradients(eng, torch.zeros(rows, dim, dtype=torch.bfloat16, device="cuda"), w, target, f32, dx=True)
+    ref = 2.0 ** -17 * w.double().sum(0)[None]
+    off = (got - ref).abs()
+    assert bool((off <= _bound(1 << 17, ref) + (0.0 if f32 else 2.0 ** -8) * ref).all()), float((off / ref).max())
