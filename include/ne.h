@@ -399,11 +399,11 @@ NE_API ne_status ne_sdpa_fwd_device(ne_ctx* ctx, const void* d_q, const void* d_
  * All calls only enqueue work on the context's stream, use the workspaces of
  * ne_head_alloc and may be captured into a graph.  dim, ldx, ldw, lddx and
  * lddw are multiples of 8, x, w, dx and dw 16-byte aligned; rows, vocab and
- * topk are arbitrary (rows may be 0, and arrays of rows then NULL).  Outputs must not overlap inputs, and are
- * the same bits every time.  The workspaces belong to one call at a time: graphs
- * of these calls are replayed one after the other.  A target or id >= vocab
- * counts as absent and is reported by the next call that synchronises
- * (NE_ERR_BOUNDS). */
+ * topk are arbitrary (rows may be 0, and arrays of rows then NULL).  Outputs
+ * must not overlap inputs, and are the same bits every time.  The workspaces
+ * belong to one call at a time: graphs of these calls are replayed one after the
+ * other.  A target or id >= vocab counts as absent and is reported by the next
+ * call that synchronises (NE_ERR_BOUNDS). */
 typedef struct ne_head_desc {
   const void* x; long long ldx;   /* bf16 [rows, dim]: hidden states after the final norm */
   const void* w; long long ldw;   /* bf16 [vocab, dim] */
@@ -419,7 +419,8 @@ typedef struct ne_teacher_desc {
   const int32_t* ids;    /* device [rows, topk] */
   const float* logits;   /* device [rows, topk] */
   int topk;
-  float temperature;     /* T: both sides' logits are divided by it; T^2 is a normal fp32 number */
+  float temperature;     /* T > 0: both sides' logits are divided by it; T^2 is
+                            a normal fp32 number */
 } ne_teacher_desc;
 
 /* Gradients to compute (NULL: not computed).  dx [rows, dim] is written, bf16
@@ -442,9 +443,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
 NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
                                 float* d_loss, float* d_lse);
 /* Gradients of sum_i grad_i loss_i, from the d_lse of ne_head_ce_fwd; d_grad
- * [rows] NULL: ones.  dz = grad (softmax - onehot) is rounded to bf16 as the
- * operand of the tensor-core products that give dx and dw; with at most 64 rows
- * that count it is kept in two bf16 parts. */
+ * [rows] NULL: ones.  dz = grad (softmax - onehot) is rounded to bf16 (2^-9 of
+ * its size), as the operand of the tensor-core products that give dx and dw, in
+ * fp32 outputs too; with at most 64 rows that count it is kept in two bf16 parts. */
 NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
                                 const float* d_lse, const float* d_grad, const ne_head_grads* g);
 

@@ -20,6 +20,8 @@
 //   backward  per piece of the vocabulary: the logits again, turned into bf16 dz
 //             by the epilogue, then dx += dz . w and dw = dz^T . x
 // Nothing is added up in an order that could change: the same bits every time.
+// Times in these files that stand side by side were measured side by side, on one
+// card; cards differ by 5 to 10%, and a later step may have moved both.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -280,7 +282,6 @@ struct HeadJoin {
   const int* pos_of;              // NULL: rows are not packed
   const int32_t* target;          // cross entropy
   const int* keep;                // distillation
-  const int* ids;
   const float* prob;
   const float* neg_entropy;
   const float* zt;
@@ -499,7 +500,8 @@ struct HeadCall {
 
 // Arrays of no rows may be NULL, as an empty array's address often is.
 ne_status head_check(ne_ctx* ctx, const ne_head_desc* d, const char* what) {
-  if ((!d->x && d->rows != 0) || !d->w) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x or w is NULL");
+  if ((!d->x && d->rows != 0) || !d->w)
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": x or w is NULL");
   if (d->rows < 0 || d->dim <= 0 || d->vocab <= 0)
     return fail(ctx, NE_ERR_INVALID, std::string(what) + ": rows, dim or vocab out of range");
   if (d->dim % 8) return fail(ctx, NE_ERR_UNSUPPORTED, std::string(what) + ": dim must be a multiple of 8");
@@ -658,7 +660,6 @@ ne_status head_forward(ne_ctx* ctx, const HeadCall& c, float* loss, float* lse) 
   j.pos_of = plan.packed ? h->pos_of : nullptr;
   j.target = c.target;
   j.keep = c.teacher ? h->keep : nullptr;
-  j.ids = h->ids;
   j.prob = h->prob;
   j.neg_entropy = h->neg_entropy;
   j.zt = h->zt;
@@ -702,13 +703,15 @@ HeadPlan head_plan(int rows, int dim, int vocab, int num_sms) {
   // of 2668 ids: 43.0 us with 8 or 6, 43.8 with 12, 45.4 with 16, 49.0 with 32; calls
   // with more to do than one unit a pair do not come to it).  dw's units cost 9
   // k-blocks at least, their epilogue.
-  const double m_tiles = (double)((rows + p.tile_m - 1) / p.tile_m), d_tiles = (dim + HB_BN - 1) / HB_BN;
+  const double m_tiles = (double)((rows + p.tile_m - 1) / p.tile_m);
+  const double d_tiles = (dim + HB_BN - 1) / HB_BN;
   const double piece_kb = p.piece / GEMM_BK;
   const double load = m_tiles * d_tiles * piece_kb +
                       (p.piece / p.tile_m) * d_tiles * std::max(9.0, (double)(rows64 / GEMM_BK));
   const double most = std::max(8.0, load / p.clusters / 2);
   const long long slabs = std::max<long long>(1, (long long)kSlabBytes / (rows64 * dim * 4));
-  const long long want = std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
+  const long long want =
+      std::max<long long>(1, std::min<long long>((long long)std::ceil(piece_kb / most), slabs));
   p.split_n = (int)up((p.piece + want - 1) / want, HB_BN);
   p.splits = (p.piece + p.split_n - 1) / p.split_n;
   // with room for it, no piece's dx waits for the piece before
@@ -807,7 +810,8 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
 }
 
 ne_status grads_check(ne_ctx* ctx, const ne_head_desc* d, const ne_head_grads* g, const char* what) {
-  if (!g->dx && !g->dw && d->rows != 0) return fail(ctx, NE_ERR_INVALID, std::string(what) + ": no gradient asked for");
+  if (!g->dx && !g->dw && d->rows != 0)
+    return fail(ctx, NE_ERR_INVALID, std::string(what) + ": no gradient asked for");
   if ((g->dx && (g->lddx < d->dim || g->lddx % 8)) || (g->dw && (g->lddw < d->dim || g->lddw % 8)))
     return fail(ctx, NE_ERR_INVALID,
                 std::string(what) + ": lddx and lddw must be multiples of 8, at least dim");
@@ -910,13 +914,15 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
     off += up(bytes, 1024);
     return at;
   };
-  const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4),
-               o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4),
-               o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8), o_lse = take(R * 4),
-               o_xp = take(R256 * up(D, GEMM_BK) * 2), o_twin = take(2 * HB_TWIN * up(D, GEMM_BK) * 2), o_target = take(R * 4), o_coef = take(R * 8),
-               o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2), o_dz = take(HB_BUFS * dz),
-               o_dx = take(std::max(R64 * D * 4, kSlabBytes)),
-               o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1) * 4);
+  const size_t o_count = take(4), o_row = take(up(R, 64) * 4), o_pos = take(R * 4);
+  const size_t o_keep = take(R * 4), o_ids = take(K * R * 4), o_prob = take(K * R * 4);
+  const size_t o_ent = take(R * 4), o_zt = take(K * R * 4), o_stats = take(pairs * 8);
+  const size_t o_lse = take(R * 4), o_xp = take(R256 * up(D, GEMM_BK) * 2);
+  const size_t o_twin = take(2 * HB_TWIN * up(D, GEMM_BK) * 2), o_target = take(R * 4);
+  const size_t o_coef = take(R * 8), o_dz = take(HB_BUFS * dz);
+  const size_t o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2);
+  const size_t o_dx = take(std::max(R64 * D * 4, kSlabBytes));
+  const size_t o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1) * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
   if (s != NE_OK) {

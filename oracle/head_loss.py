@@ -74,9 +74,10 @@ def bounds(x, w, keep, p, scale=1.0, temperature=1.0, grad=None, dz_step=2.0 ** 
     chunk sums): e = 2^-17 + 2^-22 |u|max in all.
     lse: du + e, and 2^-22 of its size; loss: T^2 times that and du more.
     dz = a (q - p): q off by q * (2 (du + e)), the value rounded to bf16, half a
-    step, dz_step = 2^-8 of its size (in two parts: 2^-16).  dx, dw: those times |w|, |x| summed, and the fp32
-    sums' own 2^-16 of the magnitudes (a step of 16 truncates 2^-23, at most
-    a few hundred steps a product here, and one fp32 addition a piece).
+    step, dz_step = 2^-8 of its size (in two parts: 2^-16).  dx, dw: those times
+    |w|, |x| summed, and the fp32 sums' own 2^-16 of the magnitudes (a step of 16
+    truncates 2^-23, at most a few hundred steps a product here, and one fp32
+    addition a piece).
     """
     T = temperature
     xs, ws, ps = x[keep].double(), w.double(), p[keep]
