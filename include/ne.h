@@ -445,7 +445,10 @@ NE_API ne_status ne_head_ce_fwd(ne_ctx* ctx, const ne_head_desc* d, const int32_
 /* Gradients of sum_i grad_i loss_i, from the d_lse of ne_head_ce_fwd; d_grad
  * [rows] NULL: ones.  dz = grad (softmax - onehot) is rounded to bf16 (2^-9 of
  * its size), as the operand of the tensor-core products that give dx and dw, in
- * fp32 outputs too; with at most 64 rows that count it is kept in two bf16 parts. */
+ * fp32 outputs too; with at most 64 rows that count it is kept in two bf16 parts.
+ * With more, what rounding takes from it at the target is added to dx and dw in
+ * fp32; dw of 32 ids (a multiple of 32 and those behind it) that are the targets
+ * of more than 32 rows goes without. */
 NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_t* d_target,
                                 const float* d_lse, const float* d_grad, const ne_head_grads* g);
 
@@ -455,7 +458,8 @@ NE_API ne_status ne_head_ce_bwd(ne_ctx* ctx, const ne_head_desc* d, const int32_
  * left out. */
 NE_API ne_status ne_head_distill_fwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
                                      float* d_loss, float* d_lse);
-/* As ne_head_ce_bwd, with dz = grad T (q - p). */
+/* As ne_head_ce_bwd, with dz = grad T (q - p); the target is the entry with the
+ * largest logit, and nothing is added for more than 4 entries a row. */
 NE_API ne_status ne_head_distill_bwd(ne_ctx* ctx, const ne_head_desc* d, const ne_teacher_desc* t,
                                      const float* d_lse, const float* d_grad,
                                      const ne_head_grads* g);

@@ -23,6 +23,11 @@
 // logits summed otherwise than the forward pass's put gradients of few rows 9e-4 off
 // (1e-4 in runs).  It costs 1 to 2% (4096 rows of 151936 ids, forward and backward:
 // 4.06 -> 4.13 ms, 256 rows of 32000 ids 74.2 -> 75.3 us).
+// dz goes into the products in bf16.  What rounding takes from it at a row's target,
+// where most of its size is, is put back in fp32: into dx by the kernel that adds the
+// slabs, into dw by the epilogue (put_back).  Gradients of 294 rows in bf16 are then
+// 1.66e-3 off float64 instead of 2.4e-3, as much as rounding them alone makes; it costs
+// 4 us of 75 at 256 rows, 7 of 281 at 1638 of 4096, 0.3% at 4096 rows of 151936 ids.
 // As launches of their own the products left 14% of the pairs idle in their last
 // waves (4096 rows, dim 1024: 64 tiles of dx, 128 of dw, for 74 pairs).
 //
@@ -43,6 +48,7 @@ constexpr int HB_THREADS = GEMM_THREADS + 32;   // warps: A, MMA, 8 x epilogue, 
 constexpr int HB_BOX = 4096;                    // 32 rows of 128 bytes
 constexpr int HB_TWIN = 64;                     // up to here rows stand twice
 constexpr int HB_TAB = 256;                     // ids per entry of a row's index
+constexpr int HB_PUT_BACK = 32;                 // rows that 32 ids' dw takes rests of, at most
 
 template <int CG>
 struct HeadCfg {
@@ -135,6 +141,13 @@ struct HeadDz {
   HeadTargets t;
   const float2* coef;   // packed rows: a, log2|a| - lse log2 e
   float c2;             // scale / (T ln 2)
+  // What rounding takes from dz at a row's largest target is put back.
+  const int* best;      // packed rows: that target's id (NULL: it is not put back)
+  float* rest;          // packed rows: what the rounding of dz there left, 0 before
+  int* rests;           // for each 32 ids: rows whose target is among them, 0 before
+  int4* list;           // for each 32 ids HB_PUT_BACK of them: row, id, rest
+  const __nv_bfloat16* x;   // packed rows
+  long long ldp;
 };
 
 struct HeadMaps {
@@ -408,9 +421,65 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// dw of 32 ids from `first`, one a lane, takes what rounding left of dz at their `n`
+// rows' targets (e: the list's place of this lane), on the accumulator: `cols` columns
+// of it, x's from n0.  An id's rows one after the other, in their order, whichever
+// entered the list first.  Called by a whole warp; a function of its own so that its
+// registers are not the epilogue's.
+__device__ __noinline__ void put_back(const HeadDz& p, int4 e, int first, int n, uint32_t taddr, int n0,
+                                      int cols) {
+  const int lane = threadIdx.x & 31;
+  int turn = 0;   // of this place among its id's
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const int row = __shfl_sync(0xffffffffu, e.x, i), id = __shfl_sync(0xffffffffu, e.y, i);
+    turn += id == e.y && row < e.x;
+  }
+  const int turns = __reduce_max_sync(0xffffffffu, lane < n ? turn : 0) + 1;
+#pragma unroll 1
+  for (int t = 0; t < turns; ++t) {
+    int row = -1;
+    float left = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int r = __shfl_sync(0xffffffffu, e.x, i), id = __shfl_sync(0xffffffffu, e.y, i);
+      const int z = __shfl_sync(0xffffffffu, e.z, i), k = __shfl_sync(0xffffffffu, turn, i);
+      if (id == first + lane && k == t) {
+        row = r;
+        left = __int_as_float(z);
+      }
+    }
+    uint4 x[16];
+    const uint4* src = reinterpret_cast<const uint4*>(p.x + (row < 0 ? 0 : row) * p.ldp + n0);
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+      x[q] = row >= 0 && 8 * q < cols ? src[q] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (32 * c >= cols) break;
+      float v[32];
+      tmem_ld32(taddr + 32 * c, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t u[4] = {x[4 * c + q].x, x[4 * c + q].y, x[4 * c + q].z, x[4 * c + q].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& a = v[8 * q + 2 * i];
+          float& b = v[8 * q + 2 * i + 1];
+          a = fmaf(left, __uint_as_float(u[i] << 16), a);
+          b = fmaf(left, __uint_as_float(u[i] & 0xffff0000u), b);
+        }
+      }
+      tmem_st32(taddr + 32 * c, v);
+    }
+    tmem_st_wait();
+  }
+}
+
 template <int CG>
 __global__ void __launch_bounds__(HB_THREADS, 1)
-head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const HeadDz dzp) {
+head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp,
+                 const __grid_constant__ HeadDz dzp) {
   using C = HeadCfg<CG>;
   constexpr bool PAIR = CG == 2;
   constexpr int TILE_M = GEMM_BM * CG;
@@ -778,9 +847,11 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       TargetCursor cur;
       float mag = 0.f, shift = 0.f;
       uint32_t keep = 0u, sign = 0u;
+      int best = -1;   // where rows stand twice nothing is left
       if (w.kind == HK_DZ) {
         const int m = (twin ? y0 & (HB_TWIN - 1) : y0) + lane;
         if (m < count) {
+          if (!twin && dzp.best) best = dzp.best[m];
           const float2 co = dzp.coef[m];
           mag = fabsf(co.x);
           shift = co.y;
@@ -803,8 +874,8 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       // 32 logits of columns n0 .. to dz.
       // dz is rounded once to bf16 by pack_bf16: it is the operand of two tensor-core
       // products.  Where rows stand twice, the second 64 take what the rounding of
-      // the first leaves: with few rows the error of one large dz (a target's) does
-      // not average out
+      // the first leaves; else what it leaves at the row's (largest) target, most of
+      // dz's size in one entry, is written down for dx and dw to take
       auto to_dz = [&](float (&v)[32], int n0) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = ex2_fast(fmaf(v[j], dzp.c2, shift));
@@ -826,6 +897,19 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
         if (twin && y0 >= HB_TWIN) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+        }
+        const int j = best - col;
+        if ((unsigned)j < 32u) {
+          float d = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i == j) d = v[i];
+          d -= __bfloat162float(__float2bfloat16_rn(d));
+          if (sign) d = -d;
+          dzp.rest[y0 + lane] = d;
+          const int at = atomicAdd(dzp.rests + best / 32, 1);
+          if (at < HB_PUT_BACK)
+            dzp.list[(best / 32) * HB_PUT_BACK + at] = make_int4(y0 + lane, best, __float_as_int(d), 0);
         }
       };
       // sends a box of 128-byte rows: 64 columns of bf16 or 32 of fp32 from column n0
@@ -881,6 +965,13 @@ head_walk_kernel(const __grid_constant__ HeadMaps maps, const HeadWalk sp, const
       // more pieces than buffers nobody asks.
       if (w.kind != HK_DZ && sp.pieces > HB_BUFS && warp == 2 && lane == 0 && crank == 0)
         flag_add(head_flag(sp, w.piece, HF_READ));
+      if (w.kind == HK_DW && !twin && dzp.best && rows_in) {
+        const int first = id0 + y0;   // the warp's ids
+        const int n = __ldcg(dzp.rests + first / 32);
+        const int4 e = __ldcg(dzp.list + first + lane);   // 32 places for 32 ids
+        if (n > 0 && n <= HB_PUT_BACK)
+          put_back(dzp, e, first, n, t_half + acc * HB_BN, n_half, min(128, sp.dim - n_half));
+      }
 #pragma unroll 1
       for (int c = 0; c < 128; c += b16 ? 64 : 32) {
         if (n_half + c >= cols_end) break;

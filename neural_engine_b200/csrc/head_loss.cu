@@ -49,7 +49,9 @@ struct HeadState {
   int* row_of = nullptr;          // packed row -> row
   int* pos_of = nullptr;          // row -> packed row, -1 where left out
   int* keep = nullptr;            // distillation: the row has an entry
-  int* target = nullptr;          // cross entropy: targets of the packed rows
+  int* target = nullptr;          // packed rows: the target, of a teacher's entries the largest
+  int* best = nullptr;            // distillation: id of a row's largest entry
+  float* rest = nullptr;          // packed rows: what rounding left of dz at the target
   float2* coef = nullptr;         // packed rows: a, log2|a| - lse log2 e
   int* ids = nullptr;             // [topk][rows] sorted, INT_MAX behind the last
   unsigned short* tab = nullptr;  // [rows][ids / 256 + 1] entries below each multiple of 256
@@ -62,7 +64,9 @@ struct HeadState {
   __nv_bfloat16* twin = nullptr;  // [128][dim up to 64] the first 64 packed rows, twice
   __nv_bfloat16* dz = nullptr;    // [3][rows up to 64][piece]
   float* dx = nullptr;            // [splits][rows up to 64][dim] sums over the pieces
-  int* counters = nullptr;        // of the backward pass: units drawn, flags of the pieces
+  int* counters = nullptr;        // of the backward pass: units drawn, flags of the pieces, rows
+                                  // with a target in each 32 ids
+  int4* list = nullptr;           // HB_PUT_BACK of them
 };
 
 namespace {
@@ -77,6 +81,12 @@ constexpr int kTopkMax = 256;
 // 0.262, 0.261, 0.245, 0.240 (32000 ids, dim 768, six rows in ten left out).
 constexpr size_t kPieceBytes = 128u << 20;
 constexpr size_t kSlabBytes = 64u << 20;
+
+// Entries a row up to which what rounding left of dz at the largest is put back: that
+// is most of the error where a row has one target (gradients of 294 rows of 71946 ids
+// off float64 by 2.4e-3 of their norm in bf16, 1.66e-3 with it, which is the output's
+// own rounding; of 4 entries 2.4e-3 and 2.2e-3, of 64 2.3e-3 and 2.2e-3 at 6% of the time).
+constexpr int kPutBackTopk = 4;
 
 inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
@@ -108,6 +118,8 @@ struct HeadPack {
   int* pos_of;
   int* count;
   int* target_p;
+  const int* best;          // distillation: by row
+  float* rest;
   __nv_bfloat16* xp;        // rows of whole 128-byte lines: what a box of 64 columns reads
   long long ldp;
   // backward
@@ -123,8 +135,7 @@ struct HeadPack {
 __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
   pdl_trigger();
   pdl_wait();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < p.n_counters; i += 256) p.counters[i] = 0;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < p.n_counters; i += gridDim.x * 256) p.counters[i] = 0;
   const int32_t* target = p.target;
   const int* keep = p.keep;
   const int rows = p.rows, vocab = p.vocab, per = p.per;
@@ -153,8 +164,9 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack p) {
       if (mine) p.pos_of[i] = on ? pos : -1;
       if (on) {
         p.row_of[pos] = i;
-        if (target) p.target_p[pos] = target[i];
+        p.target_p[pos] = target ? target[i] : p.best[i];
         if (p.coef) {
+          p.rest[pos] = 0.f;
           const float a = (p.grad ? p.grad[i] : 1.0f) * p.factor;
           p.coef[pos] = make_float2(a, log2f(fabsf(a)) - p.lse[i] * kLog2e);
         }
@@ -218,9 +230,10 @@ __device__ __forceinline__ float block_reduce(float v, float* part, int warps) {
 __global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
     const int32_t* __restrict__ ids_in, const float* __restrict__ logit, int rows, int K, int vocab,
     float temperature, int* ids, float* prob, unsigned short* tab, int tab_ld, float* neg_entropy,
-    int* keep, int* status) {
+    int* keep, int* best, int* status) {
   pdl_trigger();
   pdl_wait();
+  __shared__ int least;
   __shared__ __align__(16) unsigned sid[kTopkMax];
   __shared__ unsigned sorted[kTopkMax];
   __shared__ float part[kTopkMax / 32];
@@ -236,8 +249,10 @@ __global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
   const bool there = c >= 0 && c < vocab;
   if (!there) c = INT_MAX;
   sid[k] = (unsigned)c;
+  if (k == 0) least = INT_MAX;
   const int any = __syncthreads_or(there);
   const float top = block_reduce<true>(there ? v : -INFINITY, part, warps);
+  if (there && v == top) atomicMin(&least, c);   // of equal logits the lowest id
   // the differences are divided by T, not the logits: a logit / T may pass the range
   v = (v - top) / temperature;
   const float e = there ? expf(v) : 0.f;
@@ -268,6 +283,7 @@ __global__ void __launch_bounds__(kTopkMax) head_teacher_kernel(
   }
   if (k == 0) {
     keep[r] = any;
+    best[r] = least;
     neg_entropy[r] = ent;
   }
 }
@@ -377,11 +393,21 @@ __global__ void __launch_bounds__(256) head_join_kernel(const HeadJoin p) {
 // sums are added in the groups' order): what few rows cost is the chain of loads.
 // Forward and backward pass of 64 rows of 768 columns, 14 slabs that stand twice:
 // 62.5 us, 67.2 without groups.
+// Where rows do not stand twice, what rounding left of dz at a row's largest target
+// is put back here: times that row of w.
+struct HeadRest {
+  const int* best;              // packed rows
+  const float* rest;            // NULL: nothing is
+  const __nv_bfloat16* w;
+  long long ldw;
+};
+// (4 blocks a SM: the compiler gives the loads of eight slabs registers of their own.)
 template <class T>
-__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ acc, int slabs,
+__global__ void __launch_bounds__(256, 4) head_dx_kernel(const float* __restrict__ acc, int slabs,
                                                       long long slab, int rows, int dim, int groups,
                                                       const int* __restrict__ pos_of, T* dx,
-                                                      long long ld, int add, const int* count) {
+                                                      long long ld, int add, const int* count,
+                                                      const HeadRest p) {
   pdl_trigger();
   pdl_wait();
   __shared__ float4 part[256];
@@ -395,7 +421,14 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
   float4 v = zero;
   if (pos >= 0) {
     // where rows stand twice, the products of dz's second part lie 64 rows further
-    const int all = *count <= HB_TWIN ? 2 * slabs : slabs, each = (all + groups - 1) / groups;
+    const bool twin = *count <= HB_TWIN;
+    const int all = twin ? 2 * slabs : slabs, each = (all + groups - 1) / groups;
+    float left = 0.f;
+    int id = 0;
+    if (p.rest && !twin && g == 0) {   // on their way while the slabs are added
+      left = p.rest[pos];
+      id = p.best[pos];
+    }
     const float4* src = reinterpret_cast<const float4*>(acc + (long long)pos * dim) + k;
     const int end = min(all, (g + 1) * each);
     for (int u0 = g * each; u0 < end; u0 += 8) {
@@ -409,6 +442,13 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
       for (int u = 0; u < 8; ++u) {
         v.x += q[u].x; v.y += q[u].y; v.z += q[u].z; v.w += q[u].w;
       }
+    }
+    if (left != 0.f) {
+      const uint2 wb = *reinterpret_cast<const uint2*>(p.w + id * p.ldw + 4 * k);
+      v.x = fmaf(left, __uint_as_float(wb.x << 16), v.x);
+      v.y = fmaf(left, __uint_as_float(wb.x & 0xffff0000u), v.y);
+      v.z = fmaf(left, __uint_as_float(wb.y << 16), v.z);
+      v.w = fmaf(left, __uint_as_float(wb.y & 0xffff0000u), v.w);
     }
   }
   if (groups > 1) {
@@ -544,7 +584,8 @@ ne_status enqueue_teacher(ne_ctx* ctx, const HeadCall& c) {
   const int rows = c.d->rows;
   NE_LAUNCH(launch_k(head_teacher_kernel, dim3(rows), dim3((unsigned)up(c.n, 32)), 0, ctx->st,
                      c.teacher->ids, c.teacher->logits, rows, c.n, c.d->vocab, c.t, h->ids, h->prob,
-                     h->tab, tab_entries(c.d->vocab), h->neg_entropy, h->keep, ctx->d_status));
+                     h->tab, tab_entries(c.d->vocab), h->neg_entropy, h->keep, h->best,
+                     ctx->d_status));
   return NE_OK;
 }
 
@@ -566,6 +607,8 @@ ne_status enqueue_pack(ne_ctx* ctx, const HeadCall& c, const float* lse, const f
   p.pos_of = h->pos_of;
   p.count = h->count;
   p.target_p = h->target;
+  p.best = h->best;
+  p.rest = h->rest;
   p.xp = h->xp;
   p.ldp = (long long)up(p.dim, GEMM_BK);
   p.lse = lse;
@@ -739,14 +782,22 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
   const int rows = d.rows, V = d.vocab, D = d.dim;
   const int rows64 = std::max((int)up(rows, 64), 2 * HB_TWIN);   // few rows stand twice
   const HeadPlan plan = head_plan(rows64, D, V, ctx->num_sms);
+  const int flags = 1 + plan.pieces * (2 + plan.splits);
+  const bool put_back = c.n <= kPutBackTopk;
   ne_status s;
   if ((s = enqueue_teacher(ctx, c)) != NE_OK ||
-      (s = enqueue_pack(ctx, c, lse, grad, 1 + plan.pieces * (2 + plan.splits))) != NE_OK)
+      (s = enqueue_pack(ctx, c, lse, grad, flags + (V + 31) / 32)) != NE_OK)
     return s;
   HeadDz dz{};
   dz.t = targets_of(h, c, true);
   dz.coef = h->coef;
   dz.c2 = logit_factor(d.scale, c.t);
+  dz.best = put_back ? h->target : nullptr;
+  dz.rest = h->rest;
+  dz.rests = h->counters + flags;
+  dz.list = h->list;
+  dz.x = h->xp;
+  dz.ldp = (long long)up(D, GEMM_BK);
   const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const long long ldp = (long long)up(D, GEMM_BK);
   const int esz = g->dw_f32 ? 4 : 2, dz_rows = HB_BUFS * rows64;
@@ -797,14 +848,15 @@ ne_status head_backward(ne_ctx* ctx, const HeadCall& c, const float* lse, const 
     while (groups < 8 && loads > 8 * groups) groups *= 2;
     const int cols = 256 / groups;
     const dim3 grid((unsigned)(((long long)rows * (D / 4) + cols - 1) / cols));
+    const HeadRest rest{h->target, put_back ? h->rest : nullptr, (const __nv_bfloat16*)d.w, d.ldw};
     if (g->dx_f32)
       NE_LAUNCH(launch_k(head_dx_kernel<float>, grid, dim3(256), 0, ctx->st, (const float*)h->dx,
                          slabs, slab, rows, D, groups, (const int*)h->pos_of, (float*)g->dx, g->lddx,
-                         (int)c.add, (const int*)h->count));
+                         (int)c.add, (const int*)h->count, rest));
     else
       NE_LAUNCH(launch_k(head_dx_kernel<__nv_bfloat16>, grid, dim3(256), 0, ctx->st,
                          (const float*)h->dx, slabs, slab, rows, D, groups, (const int*)h->pos_of,
-                         (__nv_bfloat16*)g->dx, g->lddx, 0, (const int*)h->count));
+                         (__nv_bfloat16*)g->dx, g->lddx, 0, (const int*)h->count, rest));
   }
   return NE_OK;
 }
@@ -922,7 +974,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   const size_t o_coef = take(R * 8), o_dz = take(HB_BUFS * dz);
   const size_t o_tab = take(n.max_topk ? R * (size_t)tab_entries((int)V) * 2 : 2);
   const size_t o_dx = take(std::max(R64 * D * 4, kSlabBytes));
-  const size_t o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1) * 4);
+  const size_t o_counters = take((4 * (up(V, HB_BN) / HB_BN + 1) + 1 + (V + 31) / 32) * 4);
+  const size_t o_list = take((V + 31) / 32 * HB_PUT_BACK * 16);
+  const size_t o_best = take(R * 4), o_rest = take(R * 4);
   uint8_t* b = nullptr;
   ne_status s = dalloc(ctx, &b, off);
   if (s != NE_OK) {
@@ -937,6 +991,9 @@ NE_API ne_status ne_head_alloc(ne_ctx* ctx, int max_rows, int max_dim, int max_v
   n.ids = (int*)(b + o_ids);
   n.prob = (float*)(b + o_prob);
   n.target = (int*)(b + o_target);
+  n.best = (int*)(b + o_best);
+  n.rest = (float*)(b + o_rest);
+  n.list = (int4*)(b + o_list);
   n.coef = (float2*)(b + o_coef);
   n.tab = (unsigned short*)(b + o_tab);
   n.neg_entropy = (float*)(b + o_ent);
